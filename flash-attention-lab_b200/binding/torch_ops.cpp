@@ -12,6 +12,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cstdint>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -175,11 +176,173 @@ std::tuple<at::Tensor, at::Tensor> decode(const at::Tensor& q, const at::Tensor&
   return {o, lse};
 }
 
+// The KV-cache ops (flash_lab/kvcache.py, which checks shapes and dtypes before calling these).
+using OptTensor = std::optional<at::Tensor>;
+
+int cache_dtype_code(at::ScalarType t) {
+  return t == at::kChar ? static_cast<int>(FLB_INT8) : dtype_code(t, true);
+}
+
+int32_t size32(int64_t n) {
+  if (n < 0 || n > INT32_MAX) throw std::runtime_error("a size does not fit in 32 bits");
+  return static_cast<int32_t>(n);
+}
+
+const int32_t* i32_ptr(const OptTensor& t) {
+  return t.has_value() ? t->data_ptr<int32_t>() : nullptr;
+}
+
+flb_kv_cache cache_struct(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                          const at::Tensor& seq_lens, const OptTensor& block_tables,
+                          const OptTensor& k_scale, const OptTensor& v_scale) {
+  if (k_cache.dim() != 4 || v_cache.dim() != 4 || v_cache.sizes() != k_cache.sizes() ||
+      v_cache.scalar_type() != k_cache.scalar_type() || k_cache.stride(3) != 1 ||
+      v_cache.stride(3) != 1)
+    throw std::runtime_error("caches must be two alike 4-D tensors, contiguous in head_dim");
+  flb_kv_cache c{};
+  c.k_cache = k_cache.data_ptr();
+  c.v_cache = v_cache.data_ptr();
+  c.k_batch_stride = k_cache.stride(0);
+  c.k_seq_stride = k_cache.stride(1);
+  c.k_head_stride = k_cache.stride(2);
+  c.v_batch_stride = v_cache.stride(0);
+  c.v_seq_stride = v_cache.stride(1);
+  c.v_head_stride = v_cache.stride(2);
+  for (const OptTensor* s : {&k_scale, &v_scale}) {
+    if (s->has_value() && ((*s)->dim() != 3 || (*s)->sizes() != k_cache.sizes().slice(0, 3)))
+      throw std::runtime_error("scales must be [outer, rows, H_kv] like the cache");
+  }
+  if (k_scale.has_value()) {
+    c.k_scale = k_scale->data_ptr<float>();
+    c.ks_batch_stride = k_scale->stride(0);
+    c.ks_seq_stride = k_scale->stride(1);
+    c.ks_head_stride = k_scale->stride(2);
+  }
+  if (v_scale.has_value()) {
+    c.v_scale = v_scale->data_ptr<float>();
+    c.vs_batch_stride = v_scale->stride(0);
+    c.vs_seq_stride = v_scale->stride(1);
+    c.vs_head_stride = v_scale->stride(2);
+  }
+  c.batch = size32(seq_lens.numel());
+  c.heads_kv = size32(k_cache.size(2));
+  c.head_dim = size32(k_cache.size(3));
+  c.max_seqlen = size32(k_cache.size(1));
+  c.dtype = cache_dtype_code(k_cache.scalar_type());
+  if (block_tables.has_value()) {
+    if (block_tables->dim() != 2 || block_tables->size(0) != c.batch ||
+        block_tables->stride(1) != 1)
+      throw std::runtime_error("block_tables must be [B, max_blocks] int32 with unit column stride");
+    c.block_tables = block_tables->data_ptr<int32_t>();
+    c.block_table_stride = block_tables->stride(0);
+    c.page_size = size32(k_cache.size(1));
+    c.num_blocks = size32(k_cache.size(0));
+    c.max_seqlen = size32(block_tables->size(1) * k_cache.size(1));
+  } else if (k_cache.size(0) != c.batch) {
+    throw std::runtime_error("the cache and seq_lens differ in batch size");
+  }
+  return c;
+}
+
+flb_kv_rows rows_struct(const at::Tensor& k, const at::Tensor& v, const flb_kv_cache& c,
+                        const OptTensor& cu_seqlens, const at::Tensor& seq_lens,
+                        int64_t rows_per_seq) {
+  if (k.dim() != 3 || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() ||
+      k.size(1) != c.heads_kv || k.size(2) != c.head_dim || k.stride(2) != 1 || v.stride(2) != 1)
+    throw std::runtime_error("k and v must be [rows, H_kv, D], contiguous in head_dim");
+  if (cu_seqlens.has_value() && cu_seqlens->numel() != int64_t{c.batch} + 1)
+    throw std::runtime_error("cu_seqlens must be [B + 1]");
+  flb_kv_rows r{};
+  r.k = k.data_ptr();
+  r.v = v.data_ptr();
+  r.k_row_stride = k.stride(0);
+  r.k_head_stride = k.stride(1);
+  r.v_row_stride = v.stride(0);
+  r.v_head_stride = v.stride(1);
+  r.cu_seqlens = i32_ptr(cu_seqlens);
+  r.seq_lens = seq_lens.data_ptr<int32_t>();
+  r.rows = size32(k.size(0));
+  r.rows_per_seq = size32(rows_per_seq);
+  r.dtype = dtype_code(k.scalar_type(), true);
+  return r;
+}
+
+void kv_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache,
+               const at::Tensor& v_cache, const at::Tensor& seq_lens, const OptTensor& cu_seqlens,
+               const OptTensor& block_tables, const OptTensor& k_scale, const OptTensor& v_scale,
+               int64_t rows_per_seq) {
+  const c10::cuda::CUDAGuard guard(k.device());
+  const flb_kv_cache c = cache_struct(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale);
+  const flb_kv_rows r = rows_struct(k, v, c, cu_seqlens, seq_lens, rows_per_seq);
+  if (int st = flb_kv_append(&c, &r, current_stream(k))) raise_status("flb_kv_append", st);
+}
+
+std::tuple<at::Tensor, at::Tensor> kv_gather(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                             const at::Tensor& seq_lens,
+                                             const at::Tensor& cu_seqlens,
+                                             const OptTensor& block_tables,
+                                             const OptTensor& k_scale, const OptTensor& v_scale,
+                                             int64_t total, at::ScalarType dtype) {
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  const flb_kv_cache c = cache_struct(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale);
+  const auto options = k_cache.options().dtype(dtype);
+  at::Tensor k = at::empty({total, k_cache.size(2), k_cache.size(3)}, options);
+  at::Tensor v = at::empty({total, k_cache.size(2), k_cache.size(3)}, options);
+  const flb_kv_rows r = rows_struct(k, v, c, cu_seqlens, seq_lens, 0);
+  if (int st = flb_kv_gather(&c, &r, current_stream(k_cache))) raise_status("flb_kv_gather", st);
+  return {k, v};
+}
+
+std::tuple<at::Tensor, at::Tensor> extend(const at::Tensor& q, const at::Tensor& k_cache,
+                                          const at::Tensor& v_cache, const at::Tensor& seq_lens,
+                                          const OptTensor& cu_seqlens,
+                                          const OptTensor& block_tables, const OptTensor& k_scale,
+                                          const OptTensor& v_scale, int64_t rows_per_seq,
+                                          bool causal, double scale, int64_t status,
+                                          int64_t sm_count) {
+  if (q.dim() != 3 || q.stride(2) != 1)
+    throw std::runtime_error("q must be [rows, H, D], contiguous in head_dim");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const flb_kv_cache c = cache_struct(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale);
+  if (q.size(2) != c.head_dim) throw std::runtime_error("q and the cache differ in head_dim");
+  if (cu_seqlens.has_value() && cu_seqlens->numel() != int64_t{c.batch} + 1)
+    throw std::runtime_error("cu_seqlens must be [B + 1]");
+  flb_extend_params p{};
+  p.rows = size32(q.size(0));
+  p.heads = size32(q.size(1));
+  at::Tensor o = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  at::Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+  const size_t ws_bytes = flb_extend_workspace_bytes(p.rows, p.heads, c.heads_kv, c.head_dim,
+                                                     static_cast<int32_t>(sm_count));
+  at::Tensor workspace = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
+  p.q = q.data_ptr();
+  p.o = o.data_ptr();
+  p.lse = lse.data_ptr<float>();
+  p.q_row_stride = q.stride(0);
+  p.q_head_stride = q.stride(1);
+  p.o_row_stride = o.stride(0);
+  p.o_head_stride = o.stride(1);
+  p.cu_seqlens = i32_ptr(cu_seqlens);
+  p.seq_lens = seq_lens.data_ptr<int32_t>();
+  p.rows_per_seq = size32(rows_per_seq);
+  p.causal = causal ? 1 : 0;
+  p.dtype = dtype_code(q.scalar_type(), false);
+  p.softmax_scale = static_cast<float>(scale);
+  p.workspace = workspace.data_ptr();
+  p.workspace_bytes = ws_bytes;
+  p.status = reinterpret_cast<int32_t*>(status);
+  if (int st = flb_extend_fwd(&c, &p, current_stream(q))) raise_status("flb_extend_fwd", st);
+  return {o, lse};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "flash_lab's eager ops: ATen allocation + the sm_100a library's C ABI";
   m.def("prefill", &prefill, "o, lse of one prefill call (flb_prefill_fwd)");
   m.def("decode", &decode, "o, lse of one decode call (flb_decode_fwd)");
+  m.def("kv_append", &kv_append, "writes rows into a KV cache (flb_kv_append)");
+  m.def("kv_gather", &kv_gather, "k, v read back from a KV cache (flb_kv_gather)");
+  m.def("extend", &extend, "o, lse of new tokens over a KV cache (flb_extend_fwd)");
   m.def("abi_version", &flb_version);
 }

@@ -1,0 +1,80 @@
+// What the kernels of kv_cache.cu and extend.cu share: the device view of a KV cache and the map
+// from a ragged row to its sequence, and (host) the argument checks of flb_kv_cache.
+#pragma once
+
+#include <cstdint>
+
+#include "host_common.h"
+
+namespace flb {
+
+// A KV cache as the kernels see it. Strides in elements of the cache (or of the scales).
+struct KvView {
+  void* k;
+  void* v;
+  int64_t k_stride[3], v_stride[3];   // sequence or block, row, head
+  float* ks;
+  float* vs;
+  int64_t ks_stride[3], vs_stride[3];
+  const int32_t* block_tables;        // null: contiguous
+  int64_t bt_stride;
+  int page_size, num_blocks, max_seqlen, heads_kv, batch;
+
+  // The (outer, row) of key `pos` of sequence b; false when it lies outside the cache.
+  __device__ __forceinline__ bool locate(int b, int pos, int64_t& outer, int64_t& row) const {
+    if (pos < 0 || pos >= max_seqlen) return false;
+    outer = b;
+    row = pos;
+    if (block_tables != nullptr) {
+      const int page = pos / page_size;
+      const int blk = __ldg(block_tables + b * bt_stride + page);
+      if (blk < 0 || blk >= num_blocks) return false;
+      outer = blk;
+      row = pos - page * page_size;
+    }
+    return true;
+  }
+};
+
+// Ragged rows: sequence b owns rows [cu[b], cu[b + 1]), or rows_per_seq rows each (cu null).
+struct Ragged {
+  const int32_t* cu;
+  int rows, rows_per_seq, batch;
+};
+
+// The sequence that owns row t and its first row and row count; false if none does. Called by
+// whole warps with one t. cu is searched 32 ways at once: one dependent load per factor of 32 of
+// the batch.
+__device__ __forceinline__ bool find_sequence(const Ragged& r, int t, int lane, int& b, int& first,
+                                              int& count) {
+  if (r.cu == nullptr) {
+    b = t / r.rows_per_seq;
+    first = b * r.rows_per_seq;
+    count = r.rows_per_seq;
+    return b < r.batch;
+  }
+  int lo = 0, hi = r.batch;   // the answer, if any, is the largest b in [lo, hi) with cu[b] <= t
+  while (true) {
+    const int step = (hi - lo + 31) / 32;
+    const int i = lo + lane * step;
+    const bool below = i < hi && __ldg(r.cu + i) <= t;
+    const int n = __popc(__ballot_sync(0xffffffffu, below));
+    if (n == 0) return false;
+    lo += (n - 1) * step;
+    hi = min(hi, lo + step);
+    if (step == 1) break;
+  }
+  b = lo;
+  first = __ldg(r.cu + b);
+  count = __ldg(r.cu + b + 1) - first;
+  return t - first < count;
+}
+
+// Checks of an flb_kv_cache that do not depend on who uses it: required pointers, positive sizes,
+// the dtype and its scales, head_dim 64 or 128, a consistent paged layout and 16-byte aligned rows.
+int validate_kv_cache(const flb_kv_cache* c);
+KvView kv_view(const flb_kv_cache* c);
+// The [outer, rows, H_kv, D] view of the K or V array (outer: sequences or blocks).
+View4 kv_view4(const flb_kv_cache* c, bool v);
+
+}  // namespace flb

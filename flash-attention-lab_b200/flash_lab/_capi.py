@@ -1,7 +1,7 @@
 """ctypes binding of the C ABI in include/flash_lab_b200.h (libflash_lab_b200.so, built in-tree
 by flash-attention-lab_b200/build.py).
 
-The structures below mirror flb_attn_params and flb_decode_params field for field; the library
+The structures below mirror the header's parameter structs field for field; the library
 allocates nothing, so every buffer passed here comes from the caller (PyTorch's allocator in
 flash_lab.ops).
 """
@@ -26,6 +26,7 @@ FLB_ERR_NO_DEVICE = 6
 FLB_BF16 = 0
 FLB_FP16 = 1
 FLB_FP32 = 2
+FLB_INT8 = 3
 
 FLB_MAX_PEERS = 8
 
@@ -73,6 +74,44 @@ class PeerExchange(ctypes.Structure):
     ]
 
 
+class KVCache(ctypes.Structure):
+    _fields_ = [
+        ("k_cache", _p), ("v_cache", _p),
+        ("k_batch_stride", _i64), ("k_seq_stride", _i64), ("k_head_stride", _i64),
+        ("v_batch_stride", _i64), ("v_seq_stride", _i64), ("v_head_stride", _i64),
+        ("k_scale", _p), ("v_scale", _p),
+        ("ks_batch_stride", _i64), ("ks_seq_stride", _i64), ("ks_head_stride", _i64),
+        ("vs_batch_stride", _i64), ("vs_seq_stride", _i64), ("vs_head_stride", _i64),
+        ("block_tables", _p), ("block_table_stride", _i64),
+        ("page_size", _i32), ("num_blocks", _i32),
+        ("batch", _i32), ("heads_kv", _i32), ("head_dim", _i32), ("max_seqlen", _i32),
+        ("dtype", _i32),
+    ]
+
+
+class KVRows(ctypes.Structure):
+    _fields_ = [
+        ("k", _p), ("v", _p),
+        ("k_row_stride", _i64), ("k_head_stride", _i64),
+        ("v_row_stride", _i64), ("v_head_stride", _i64),
+        ("cu_seqlens", _p), ("seq_lens", _p),
+        ("rows", _i32), ("rows_per_seq", _i32), ("dtype", _i32),
+    ]
+
+
+class ExtendParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _p), ("o", _p), ("lse", _p),
+        ("q_row_stride", _i64), ("q_head_stride", _i64),
+        ("o_row_stride", _i64), ("o_head_stride", _i64),
+        ("cu_seqlens", _p), ("seq_lens", _p),
+        ("rows", _i32), ("rows_per_seq", _i32), ("heads", _i32),
+        ("causal", _i32), ("dtype", _i32), ("softmax_scale", ctypes.c_float),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_size_t),
+        ("status", _p),
+    ]
+
+
 # Every symbol include/flash_lab_b200.h declares, with its ctypes signature.
 SIGNATURES = {
     "flb_version": ([], ctypes.c_int),
@@ -100,6 +139,10 @@ SIGNATURES = {
     "flb_decode_merge_peers": ([ctypes.POINTER(PeerExchange), _i32, _i32, _i32, _i32, _i32, _p,
                                 _i64, _i64, _p, _p, _p], ctypes.c_int),
     "flb_peer_exchange_reset": ([ctypes.POINTER(PeerExchange), _p], ctypes.c_int),
+    "flb_kv_append": ([ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), _p], ctypes.c_int),
+    "flb_kv_gather": ([ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), _p], ctypes.c_int),
+    "flb_extend_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32], ctypes.c_size_t),
+    "flb_extend_fwd": ([ctypes.POINTER(KVCache), ctypes.POINTER(ExtendParams), _p], ctypes.c_int),
 }
 
 _LIB: ctypes.CDLL | None = None

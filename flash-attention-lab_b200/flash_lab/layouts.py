@@ -159,3 +159,109 @@ def check_decode_inputs(q, k_cache, v_cache, seq_lens, block_tables=None, *,
     if require_unit_stride:
         _check_unit_stride({"q": q, "k_cache": k_cache, "v_cache": v_cache})
     return q, DecodeShape(batch, heads, heads_kv, head_dim, max_seqlen, page_size)
+
+
+@dataclass(frozen=True)
+class CacheShape:
+    batch: int
+    heads_kv: int
+    head_dim: int
+    max_seqlen: int  # S_max of a contiguous cache, max_blocks * page_size of a paged one
+    page_size: int   # 0 for a contiguous cache
+    int8: bool
+
+
+def check_cache_inputs(k_cache, v_cache, seq_lens, block_tables=None, k_scale=None, v_scale=None,
+                       cu_seqlens=None, others: dict | None = None) -> CacheShape:
+    """A KV cache (as in check_decode_inputs) whose type may also be int8 with one fp32 scale per
+    token and KV head, the lengths of its sequences and the offsets of ragged rows. `others` are
+    further tensors of the call, which must be on the same device."""
+    named = {"k_cache": k_cache, "v_cache": v_cache, "seq_lens": seq_lens}
+    for name, x in (("block_tables", block_tables), ("k_scale", k_scale), ("v_scale", v_scale),
+                    ("cu_seqlens", cu_seqlens), *(others or {}).items()):
+        if x is not None:
+            named[name] = x
+    for name, x in named.items():
+        _require_tensor(name, x)
+    if len({x.device for x in named.values()}) != 1:
+        devices = {name: str(x.device) for name, x in named.items()}
+        raise ValueError(f"cache inputs must be on one device, got {devices}")
+    if k_cache.dim() != 4:
+        raise ValueError(f"k_cache must be 4-D, got shape {tuple(k_cache.shape)}")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError(
+            f"k_cache and v_cache must have the same shape, "
+            f"got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}"
+        )
+    if k_cache.dtype != v_cache.dtype:
+        raise TypeError(
+            f"k_cache and v_cache must share a dtype, got {k_cache.dtype}, {v_cache.dtype}"
+        )
+    int8 = k_cache.dtype == torch.int8
+    if (k_scale is None) == int8 or (v_scale is None) == int8:
+        raise ValueError("int8 caches need k_scale and v_scale, other caches take neither")
+    for name, x in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if x is None:
+            continue
+        if x.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32, got {x.dtype}")
+        if x.shape != k_cache.shape[:3]:
+            raise ValueError(
+                f"{name} must have shape {tuple(k_cache.shape[:3])}, got {tuple(x.shape)}"
+            )
+    for name, x in (("seq_lens", seq_lens), ("cu_seqlens", cu_seqlens)):
+        if x is None:
+            continue
+        if x.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32, got {x.dtype}")
+        if x.dim() != 1:
+            raise ValueError(f"{name} must be 1-D, got shape {tuple(x.shape)}")
+        if not x.is_contiguous():
+            raise ValueError(f"{name} must be contiguous, got stride {x.stride()}")
+    batch = seq_lens.shape[0]
+    if cu_seqlens is not None and cu_seqlens.shape[0] != batch + 1:
+        raise ValueError(
+            f"cu_seqlens must have shape ({batch + 1},), got {tuple(cu_seqlens.shape)}"
+        )
+    if block_tables is None:
+        batch_c, max_seqlen, heads_kv, head_dim = k_cache.shape
+        page_size = 0
+        if batch_c != batch:
+            raise ValueError(f"batch size mismatch: seq_lens has {batch}, the cache has {batch_c}")
+    else:
+        if block_tables.dtype != torch.int32:
+            raise TypeError(f"block_tables must be int32, got {block_tables.dtype}")
+        if block_tables.dim() != 2 or block_tables.shape[0] != batch:
+            raise ValueError(
+                f"block_tables must be [{batch}, max_blocks], got {tuple(block_tables.shape)}"
+            )
+        if block_tables.stride(1) != 1:
+            raise ValueError(f"block_tables must be contiguous in its last dimension, "
+                             f"got strides {tuple(block_tables.stride())}")
+        _, page_size, heads_kv, head_dim = k_cache.shape
+        max_seqlen = block_tables.shape[1] * page_size
+    if min(k_cache.numel(), batch, max_seqlen) == 0:
+        raise ValueError(f"empty input: k_cache {tuple(k_cache.shape)}, {batch} sequences")
+    _check_unit_stride({"k_cache": k_cache, "v_cache": v_cache})
+    return CacheShape(batch, heads_kv, head_dim, max_seqlen, page_size, int8)
+
+
+def ragged_rows(name: str, x, batch: int, cu_seqlens):
+    """x as [rows, H, D] and the rows per sequence (0: they come from cu_seqlens). With
+    cu_seqlens x is [T, H, D]; without it x is [B, n, H, D], or [B, H, D] for one row each."""
+    _require_tensor(name, x)
+    if cu_seqlens is not None:
+        if x.dim() != 3:
+            raise ValueError(f"{name} must be [T, H, D] with cu_seqlens, got shape {tuple(x.shape)}")
+        rows, per_seq = x, 0
+    elif x.dim() in (3, 4):
+        if x.shape[0] != batch:
+            raise ValueError(f"batch size mismatch: {name} has {x.shape[0]}, seq_lens has {batch}")
+        per_seq = 1 if x.dim() == 3 else x.shape[1]
+        rows = x if x.dim() == 3 else x.flatten(0, 1)
+    else:
+        raise ValueError(f"{name} must be [B, n, H, D] or [B, H, D], got shape {tuple(x.shape)}")
+    if rows.numel() == 0:
+        raise ValueError(f"empty input: {name} {tuple(x.shape)}")
+    _check_unit_stride({name: x})
+    return rows, per_seq

@@ -467,7 +467,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
 
 def decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seq_lens: torch.Tensor,
            block_tables: torch.Tensor | None = None, softmax_scale: float | None = None,
-           impl: str = "auto", num_splits: int | None = None, return_lse: bool = False):
+           impl: str = "auto", num_splits: int | None = None, return_lse: bool = False,
+           k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None):
     """One decode step: each sequence's single query token attends to its first seq_lens[b] keys.
 
     The cache is [B, S_max, H_kv, D], read in place through its strides, or paged:
@@ -475,7 +476,17 @@ def decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seq_le
     32 or a multiple of 64). seq_lens values are not checked on the host (that would force a device
     sync); the kernel clamps them to [0, S_max].
     num_splits=None lets the library choose the split count from the shapes only.
+
+    An int8 cache (flash_lab.kvcache) comes with its k_scale and v_scale; q is then bf16 or fp16, and
+    impl and num_splits stay at their defaults.
     """
+    if k_scale is not None or v_scale is not None:
+        from flash_lab import kvcache
+
+        if impl != "auto" or num_splits is not None:
+            raise ValueError("decode over an int8 cache takes no impl or num_splits")
+        return kvcache.decode_int8(q, k_cache, v_cache, seq_lens, block_tables, softmax_scale,
+                                   k_scale, v_scale, return_lse)
     fast_key = None
     if (_NATIVE is not None and block_tables is None and not DEBUG and type(q) is torch.Tensor
             and type(k_cache) is torch.Tensor and type(v_cache) is torch.Tensor

@@ -51,8 +51,9 @@ typedef enum {
   FLB_ERR_NO_DEVICE = 6         /* no sm_100 device current */
 } flb_status;
 
-/* FLB_FP32 is accepted by the decode entry points only (the reference's fp32 decode). */
-typedef enum { FLB_BF16 = 0, FLB_FP16 = 1, FLB_FP32 = 2 } flb_dtype;
+/* FLB_FP32 is accepted by the decode and cache entry points only (the reference's fp32 decode);
+ * FLB_INT8 only as the type of an flb_kv_cache. */
+typedef enum { FLB_BF16 = 0, FLB_FP16 = 1, FLB_FP32 = 2, FLB_INT8 = 3 } flb_dtype;
 
 /*
  * Prefill problem. Mirrors AttnParams (csrc/common/params.h:9-27 of the reference).
@@ -270,6 +271,96 @@ int flb_decode_merge_peers(const flb_peer_exchange* exchange, int32_t batch, int
 /* Zeroes this rank's counter block (arrivals, CTA counts, step count) on `stream`. Collective in
  * effect: every rank resets, with no push or merge of any rank in flight, before the next step. */
 int flb_peer_exchange_reset(const flb_peer_exchange* exchange, flb_stream_t stream);
+
+/*
+ * KV cache of a serving loop: written by flb_kv_append, read back by flb_kv_gather and attended to
+ * by flb_extend_fwd (and, at 16 or 32 bits, by flb_decode_fwd). No counterpart in the reference,
+ * which takes a cache that something else has filled.
+ * k_cache / v_cache are [B, S_max, H_kv, D] with k_batch_stride the sequence stride, or paged as in
+ * flb_decode_params when block_tables is not NULL ([num_blocks, page_size, H_kv, D],
+ * k_batch_stride the block stride, max_seqlen = max_blocks * page_size).
+ * dtype FLB_INT8: row x of D values (one token, one KV head) is stored as the codes
+ * q = round(x * min(127 / max|x|, 2^100)) (to nearest even) and the fp32 scale
+ * s = max(max|x| / 127, 2^-100), and stands for q * s. A row with a non-finite value is stored as
+ * zeros with a NaN scale and reads back as NaN. k_scale / v_scale hold one scale per token and KV
+ * head, [B, S_max, H_kv] (or [num_blocks, page_size, H_kv]) with any strides; NULL otherwise.
+ * All strides are in elements.
+ */
+typedef struct {
+  void* k_cache;
+  void* v_cache;
+  int64_t k_batch_stride, k_seq_stride, k_head_stride;
+  int64_t v_batch_stride, v_seq_stride, v_head_stride;
+  float* k_scale;
+  float* v_scale;
+  int64_t ks_batch_stride, ks_seq_stride, ks_head_stride;
+  int64_t vs_batch_stride, vs_seq_stride, vs_head_stride;
+  const int32_t* block_tables;
+  int64_t block_table_stride;
+  int32_t page_size, num_blocks;
+  int32_t batch, heads_kv, head_dim, max_seqlen;
+  int32_t dtype;         /* flb_dtype */
+} flb_kv_cache;
+
+/*
+ * Ragged rows of K and V outside the cache, [rows, H_kv, D] each: sequence b owns rows
+ * cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (cu_seqlens [B + 1] int32 on the device, never read on
+ * the host), or rows b * rows_per_seq .. (b + 1) * rows_per_seq - 1 when cu_seqlens is NULL.
+ * seq_lens [B] int32 counts each sequence's keys in the cache.
+ */
+typedef struct {
+  void* k;
+  void* v;
+  int64_t k_row_stride, k_head_stride;
+  int64_t v_row_stride, v_head_stride;
+  const int32_t* cu_seqlens;
+  const int32_t* seq_lens;
+  int32_t rows, rows_per_seq;
+  int32_t dtype;         /* FLB_BF16, FLB_FP16 or FLB_FP32 */
+} flb_kv_rows;
+
+/* Writes each sequence's rows into the cache at its last positions: with n rows, row i of sequence
+ * b becomes key seq_lens[b] - n + i. Rows that belong to no sequence, positions outside
+ * [0, max_seqlen) and block ids outside [0, num_blocks) are skipped. An FLB_INT8 cache is quantised
+ * as it is written; any other cache has the rows' dtype. Two rows that name the same cache row race. */
+int flb_kv_append(const flb_kv_cache* cache, const flb_kv_rows* rows, flb_stream_t stream);
+
+/* Reads sequences back: row i of sequence b becomes key i of sequence b, in the rows' dtype (the
+ * cache's own unless it is FLB_INT8). Keys at or past seq_lens[b], block ids outside
+ * [0, num_blocks) and rows that belong to no sequence give zeros. */
+int flb_kv_gather(const flb_kv_cache* cache, const flb_kv_rows* rows, flb_stream_t stream);
+
+/*
+ * Attention of new tokens over the cache that already holds their K and V. q and o are
+ * [rows, H, D] (dtype FLB_BF16 or FLB_FP16; the cache has the same dtype or FLB_INT8), ragged like
+ * flb_kv_rows; lse is [rows, H] fp32. Sequence b has L = seq_lens[b] keys (clamped to
+ * [0, max_seqlen]) and its n rows are its last n tokens: row i sees keys 0 .. L - n + i when
+ * causal is 1, all L keys otherwise. Rows that see no key or belong to no sequence give 0 and
+ * an LSE of -inf. head_dim 64 or 128, H / H_kv at most 128, pages of 8, 16, 32 or a multiple of
+ * 64 rows; pointers and strides of q, o and the caches are multiples of 16 bytes.
+ * workspace holds flb_extend_workspace_bytes(...) bytes; nothing in it needs initialising.
+ */
+typedef struct {
+  const void* q;
+  void* o;
+  float* lse;
+  int64_t q_row_stride, q_head_stride;
+  int64_t o_row_stride, o_head_stride;
+  const int32_t* cu_seqlens;
+  const int32_t* seq_lens;
+  int32_t rows, rows_per_seq, heads;
+  int32_t causal;        /* 0 or 1 */
+  int32_t dtype;         /* flb_dtype */
+  float softmax_scale;   /* > 0 */
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* status;       /* optional device status word */
+} flb_extend_params;
+
+size_t flb_extend_workspace_bytes(int32_t rows, int32_t heads, int32_t heads_kv, int32_t head_dim,
+                                  int32_t sm_count);
+int flb_extend_fwd(const flb_kv_cache* cache, const flb_extend_params* params,
+                   flb_stream_t stream);
 
 /*
  * Unit test of the tcgen05 building blocks the prefill kernel uses (no reference counterpart;
