@@ -160,6 +160,7 @@ int encode_rows_map(CUtensorMap* map, TmaCoords* coords, const View4& v, int box
   coords->pad = 0;
   const CUtensorMapDataType type =
       dtype == FLB_FP32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+      : dtype == FLB_INT8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
       : dtype == FLB_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUresult r = encode(map, type, 4, const_cast<void*>(v.base), dims, strides, box, elem_strides,
@@ -235,6 +236,41 @@ int encode_rows_x64x2_map(CUtensorMap* map, TmaCoords* coords, const View4& v, i
                 (unsigned long long)dims[4], (unsigned long long)strides[0],
                 (unsigned long long)strides[1], (unsigned long long)strides[2],
                 (unsigned long long)strides[3]);
+  }
+  return FLB_OK;
+}
+
+int encode_group_map(CUtensorMap* map, const void* base, int64_t rows, int heads_kv, int group,
+                     int head_dim, int64_t row_stride, int64_t head_stride, int box_rows,
+                     int dtype) {
+  auto encode = encoder();
+  if (encode == nullptr) {
+    return fail(FLB_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable (%s)",
+                cudaGetErrorString(g_encode_err));
+  }
+  // Size-1 dimensions may have any stride: they get a harmless multiple of 16 bytes.
+  const bool one_head = group == 1 && heads_kv == 1;
+  const cuuint64_t head = one_head ? 16 : static_cast<cuuint64_t>(head_stride * 2);
+  const cuuint64_t row = rows == 1 ? 16 : static_cast<cuuint64_t>(row_stride * 2);
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(group),
+                              static_cast<cuuint64_t>(heads_kv), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[3] = {head, head * static_cast<cuuint64_t>(group), row};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(group), 1,
+                             static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t elem_strides[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type =
+      dtype == FLB_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = encode(map, type, 4, const_cast<void*>(base), dims, strides, box, elem_strides,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    return fail(FLB_ERR_CUDA,
+                "cuTensorMapEncodeTiled failed (%d): dims %llu,%llu,%llu,%llu strides "
+                "%llu,%llu,%llu bytes",
+                static_cast<int>(r), (unsigned long long)dims[0], (unsigned long long)dims[1],
+                (unsigned long long)dims[2], (unsigned long long)dims[3],
+                (unsigned long long)strides[0], (unsigned long long)strides[1],
+                (unsigned long long)strides[2]);
   }
   return FLB_OK;
 }

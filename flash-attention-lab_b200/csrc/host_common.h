@@ -56,6 +56,13 @@ int encode_rows_map(CUtensorMap* map, TmaCoords* coords, const View4& v, int box
 int encode_rows_x64x2_map(CUtensorMap* map, TmaCoords* coords, const View4& v, int box_rows,
                           int dtype);
 
+// A map over 16-bit query rows [rows, heads_kv * group, head_dim] whose box is box_rows rows x the
+// group of one KV head x 64 columns, 128-byte swizzled: smem row i * group + h is head h of row i.
+// Coordinates: column, 0, KV head, row.
+int encode_group_map(CUtensorMap* map, const void* base, int64_t rows, int heads_kv, int group,
+                     int head_dim, int64_t row_stride, int64_t head_stride, int box_rows,
+                     int dtype);
+
 // The 16-byte row rule every kernel here relies on: base pointer and every stride of a dimension
 // longer than 1 are multiples of 16 bytes, and the head_dim stride is 1.
 bool rows_16b_aligned(const View4& v);
