@@ -1360,8 +1360,8 @@ int build_maps(const flb_decode_params* p, CUtensorMap* tmk, CUtensorMap* tmv, T
     return fail(FLB_ERR_MISALIGNED, "v_cache must have 16-byte aligned rows (data pointer and strides)");
   const int box_rows = box_rows_for(p);
   if (p->dtype == FLB_FP32) {   // [box_rows x D] fp32 boxes, unswizzled
-    if (int st = encode_rows_map(tmk, kc, kv, box_rows, p->head_dim, FLB_FP32, false)) return st;
-    return encode_rows_map(tmv, vc, vv, box_rows, p->head_dim, FLB_FP32, false);
+    if (int st = encode_rows_map(tmk, kc, kv, box_rows, p->head_dim, FLB_FP32, 0)) return st;
+    return encode_rows_map(tmv, vc, vv, box_rows, p->head_dim, FLB_FP32, 0);
   }
   if (uses_halves_map(p)) {
     if (int st = encode_rows_x64x2_map(tmk, kc, kv, box_rows, p->dtype)) return st;

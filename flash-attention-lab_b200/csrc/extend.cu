@@ -42,35 +42,33 @@
 #include <cstdint>
 #include <type_traits>
 
-#include "kv_cache.cuh"
-#include "sm100.cuh"
+#include "extend_work.cuh"
 
 namespace flb {
 namespace {
 
 constexpr int kBM = 128;              // score rows per tile
-constexpr int kBN = 128;              // keys per tile
 constexpr int kBoxBytes = kBM * 128;  // a swizzled [128 rows x 64 columns] 16-bit box
 constexpr uint32_t kTmemCols = 512;   // S0 | S1 | O0 | O1
-constexpr float kRescaleThreshold = 8.0f;   // log2 units: weights stay <= 2^8
-constexpr int kItemUnits = 2;         // fixed cost of an item, in halves of a two-tile key tile
-constexpr int kMaxBatch = 8192;       // the units' prefix sums use the K/V ring before it fills
-constexpr float kMinScale = 0x1p-100f;
-constexpr int kMaxCtas = 256;         // SMs of a device (one CTA each)
 constexpr int kScaleSlots = 4;        // key tiles whose scales are held (see the converter)
 
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr int kConvertWarp = 12;      // int8: warps 12-15
 
-// 16-bit: 128 KB of K/V tiles beside the two Q tiles. int8: 96 KB of 16-bit tiles, 48 KB of codes.
+// 16-bit: 128 KB of K/V tiles beside the two Q tiles. int8: 96 KB of 16-bit tiles, 48 KB of codes
+// (what is in flight from HBM). K and V have rings of their own, and K runs one tile ahead of V:
+// with 96 KB in one ring the next K tile waited for the last P V, and the MMA warp with it, which
+// put both chains in line (8 sequences of 24K int8 keys, one row: 297 us).
 template <int D, bool kInt8>
 struct Geometry {
   static_assert(D == 64 || D == 128, "head_dim 64 or 128");
   static constexpr int kBoxes = D / 64;
   static constexpr int kTileBytes = kBM * D * 2;
   static constexpr int kCodeBytes = kBN * D;
-  static constexpr int kSlots = (kInt8 ? 3 : 4) * (128 / D);
+  static constexpr int kKSlots = 2 * (128 / D);
+  static constexpr int kVSlots = (kInt8 ? 1 : 2) * (128 / D);
+  static constexpr int kSlots = kKSlots + kVSlots;
   static constexpr int kCodeSlots = kInt8 ? 3 * (128 / D) : 0;
   static constexpr int kScaleBytes = kInt8 ? kScaleSlots * 3 * kBN * 4 : 0;
   static constexpr int kRingOffset = 2 * kTileBytes;
@@ -87,35 +85,14 @@ struct Geometry {
   static_assert((kMaxBatch + 1) * 8 <= kSlots * kTileBytes, "prefix sums fit in the ring");
 };
 
-struct ExtendArgs {
-  void* o;
-  float* lse;
-  int64_t o_stride[2];                // row, head
-  const int32_t* seq_lens;
-  Ragged ragged;
-  int* status;
-  int heads, group, causal;
-  int tile_tokens;                    // tokens per tile: 128 / group
-  int box_rows;                       // cache rows per TMA box (a box never crosses a page)
-  float scale_log2;
-  TmaCoords kc, vc;
-  // Partials: slot 2 c + i is CTA c's first (0) or last (1) item share. part_o holds
-  // [slots][D / 8][part_rows][8], part_ml [slots][part_rows][2].
-  int part_rows;
-  float* part_o;
-  float* part_ml;
-  int4* part_meta;                    // [slots]: flags, first token's row, tokens, KV head
-  KvView cache;
-};
-
-enum : int { kPartValid = 1, kPartOpens = 2, kPartCloses = 4 };
-
-template <int kSlots, int kCodeSlots>
+template <int kKSlots, int kVSlots, int kCodeSlots>
 struct Shared {
   uint64_t q_full[2];
   uint64_t q_free[2];        // the last Q K^T of an item that reads a Q tile has completed
-  uint64_t kv_full[kSlots];
-  uint64_t kv_empty[kSlots];
+  uint64_t k_full[kKSlots];
+  uint64_t k_empty[kKSlots];
+  uint64_t v_full[kVSlots];
+  uint64_t v_empty[kVSlots];
   uint64_t code_full[kCodeSlots + 1];
   uint64_t code_empty[kCodeSlots + 1];
   uint64_t scale_full[kScaleSlots];
@@ -126,221 +103,9 @@ struct Shared {
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort_flag;
-  int start[4];              // where this CTA's share starts: sequence, KV head, item, unit in it
-  int64_t units;             // and how long it is
+  Share share;
   float2 x_ml[kBM];          // (m, l) of the second chain's rows
 };
-
-__device__ __forceinline__ int tma_c(const TmaCoords& c, int slot, int s, int h, int b) {
-  return c.pos_s == slot ? s : (c.pos_h == slot ? h : b);
-}
-
-// --------------------------------------------------------------------------------------------
-// The work
-// --------------------------------------------------------------------------------------------
-
-struct Sequence {
-  int row0, n, len;   // first row, rows, keys
-};
-
-__device__ __forceinline__ Sequence load_sequence(const ExtendArgs& a, int b) {
-  Sequence s;
-  const Ragged& r = a.ragged;
-  int end;
-  if (r.cu != nullptr) {
-    s.row0 = min(max(__ldg(r.cu + b), 0), r.rows);
-    end = min(max(__ldg(r.cu + b + 1), s.row0), r.rows);
-  } else {
-    s.row0 = static_cast<int>(min(static_cast<int64_t>(b) * r.rows_per_seq,
-                                  static_cast<int64_t>(r.rows)));
-    end = s.row0 + min(r.rows_per_seq, r.rows - s.row0);
-  }
-  s.n = end - s.row0;
-  s.len = min(max(__ldg(a.seq_lens + b), 0), a.cache.max_seqlen);
-  return s;
-}
-
-// Key tiles that the first `tokens` rows of a sequence see.
-__device__ __forceinline__ int tiles_seen(const ExtendArgs& a, const Sequence& s, int tokens) {
-  const int keys = a.causal ? min(s.len, s.len - s.n + tokens) : s.len;
-  return keys <= 0 ? 0 : (keys + kBN - 1) / kBN;
-}
-
-// Item k of a sequence: tokens [k 2 tt, (k + 1) 2 tt). Its cost in units.
-__device__ __forceinline__ int items_of(const ExtendArgs& a, const Sequence& s) {
-  return (s.n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens);
-}
-__device__ __forceinline__ int item_units(const ExtendArgs& a, const Sequence& s, int k) {
-  const int first = k * 2 * a.tile_tokens;
-  const int last = min(first + 2 * a.tile_tokens, s.n);
-  const int weight = last - first <= a.tile_tokens ? 1 : 2;
-  return kItemUnits + weight * tiles_seen(a, s, last);
-}
-
-// A CTA's part of an item: key tiles [t0, t1) of all `tiles`.
-struct Segment {
-  Sequence seq;
-  int b, hkv, first, tokens;   // sequence, KV head, first token in it, tokens
-  int t0, t1, tiles;
-  bool dual;                   // the tokens fit in one tile
-  int count[2];                // key tiles each chain runs here
-
-  // Chain c's j-th key tile.
-  __device__ __forceinline__ int tile(int c, int j) const { return dual ? t0 + 2 * j + c : t0 + j; }
-  // Its place in this segment's ring order.
-  __device__ __forceinline__ int place(int c, int j) const { return dual ? 2 * j + c : j; }
-};
-
-// Walks a CTA's share segment by segment; every role walks the same sequence of segments.
-struct Walk {
-  Sequence seq;
-  int b, hkv, k, at;
-  int64_t left;
-
-  template <typename Sh>
-  __device__ __forceinline__ void start(const ExtendArgs& a, const Sh* sh) {
-    b = sh->start[0];
-    hkv = sh->start[1];
-    k = sh->start[2];
-    at = sh->start[3];
-    left = sh->units;
-    if (left > 0) seq = load_sequence(a, b);
-  }
-
-  __device__ __forceinline__ bool next(const ExtendArgs& a, Segment& s) {
-    while (left > 0) {
-      const int per_item = 2 * a.tile_tokens;
-      s.seq = seq;
-      s.b = b;
-      s.hkv = hkv;
-      s.first = k * per_item;
-      s.tokens = min(per_item, seq.n - s.first);
-      s.dual = s.tokens <= a.tile_tokens;
-      s.tiles = tiles_seen(a, seq, s.first + s.tokens);
-      const int weight = s.dual ? 1 : 2;
-      const int total = kItemUnits + weight * s.tiles;
-      const int from = at;
-      const int to = static_cast<int>(min(static_cast<int64_t>(total), at + left));
-      s.t0 = (max(from - kItemUnits, 0) + weight - 1) / weight;
-      s.t1 = (max(to - kItemUnits, 0) + weight - 1) / weight;
-      left -= to - from;
-      at = to;
-      if (to == total) {
-        at = 0;
-        if (++k >= items_of(a, seq)) {
-          k = 0;
-          if (++hkv >= a.cache.heads_kv) {
-            hkv = 0;
-            if (left > 0) {
-              do {
-                seq = load_sequence(a, ++b);
-              } while (seq.n == 0);   // some later sequence has rows: units are left
-            }
-          }
-        }
-      }
-      if (s.t1 > s.t0 || (s.tiles == 0 && from == 0)) {
-        const int n = s.t1 - s.t0;
-        if (s.dual) {
-          s.count[0] = (n + 1) / 2;
-          s.count[1] = n / 2;
-        } else {
-          s.count[0] = min(max(tiles_seen(a, s.seq, s.first + a.tile_tokens), s.t0), s.t1) - s.t0;
-          s.count[1] = n;
-        }
-        return true;
-      }
-    }
-    return false;
-  }
-};
-
-// Finds this CTA's share. All threads; `pref` is shared memory for batch + 1 values.
-template <typename Sh>
-__device__ __forceinline__ void find_share(const ExtendArgs& a, Sh* sh, int64_t* pref) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int batch = a.ragged.batch;
-  constexpr int kFew = 4;   // items one thread sums by itself
-  for (int b = threadIdx.x; b < batch; b += blockDim.x) {
-    const Sequence s = load_sequence(a, b);
-    const int n = items_of(a, s);
-    int64_t sum = 0;
-    for (int k = 0; k < min(n, kFew); ++k) sum += item_units(a, s, k);
-    pref[b] = n > kFew ? -1 : sum * a.cache.heads_kv;
-  }
-  __syncthreads();
-  for (int b = warp; b < batch; b += blockDim.x >> 5) {
-    if (pref[b] != -1) continue;
-    const Sequence s = load_sequence(a, b);
-    const int n = items_of(a, s);
-    int64_t sum = 0;
-    for (int k = lane; k < n; k += 32) sum += item_units(a, s, k);
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    __syncwarp();
-    if (lane == 0) pref[b] = sum * a.cache.heads_kv;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    // Exclusive prefix sums in place; pref[batch] is the total.
-    int64_t run = 0;
-    for (int b0 = 0; b0 < batch; b0 += 32) {
-      const int64_t own = b0 + lane < batch ? pref[b0 + lane] : 0;
-      int64_t incl = own;
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      if (b0 + lane < batch) pref[b0 + lane] = run + incl - own;
-      run += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    __syncwarp();
-    const int64_t total = run;
-    const int64_t g0 = total * blockIdx.x / gridDim.x;
-    const int64_t g1 = total * (blockIdx.x + 1) / gridDim.x;
-    if (g1 > g0) {
-      // The largest b with pref[b] <= g0 (sequences without rows share their successor's start).
-      int lo = 0, hi = batch - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (pref[mid] <= g0) lo = mid;
-        else hi = mid - 1;
-      }
-      const Sequence s = load_sequence(a, lo);
-      const int64_t own = (lo + 1 < batch ? pref[lo + 1] : total) - pref[lo];
-      const int64_t per_head = own / a.cache.heads_kv;
-      int64_t rem = g0 - pref[lo];
-      const int hkv = static_cast<int>(rem / per_head);
-      rem -= hkv * per_head;
-      // The item that holds unit rem of this (sequence, head).
-      const int n = items_of(a, s);
-      int64_t before = 0;
-      int k = 0;
-      for (int k0 = 0; k0 < n; k0 += 32) {
-        const int64_t u = k0 + lane < n ? item_units(a, s, k0 + lane) : 0;
-        int64_t incl = u;
-        for (int o = 1; o < 32; o <<= 1) {
-          const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += v;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, before + incl > rem);
-        if (past != 0) {
-          const int at = __ffs(past) - 1;
-          before += __shfl_sync(0xffffffffu, incl - u, at);
-          k = k0 + at;
-          break;
-        }
-        before += __shfl_sync(0xffffffffu, incl, 31);
-      }
-      if (lane == 0) {
-        sh->start[0] = lo;
-        sh->start[1] = hkv;
-        sh->start[2] = k;
-        sh->start[3] = static_cast<int>(rem - before);
-      }
-    }
-    if (lane == 0) sh->units = g1 - g0;
-  }
-}
 
 // --------------------------------------------------------------------------------------------
 // Operand descriptors (see prefill.cu: any tile and k-step is one add to a base descriptor)
@@ -365,51 +130,33 @@ constexpr uint32_t mnmajor_step(int kk) { return kk * 2048; }
 // 8-bit codes
 // --------------------------------------------------------------------------------------------
 
-// Four codes as two pairs of exact bf16 or fp16 values. fp16: the byte 128 + q in the low bits of
-// 1024 is 1152 + q. bf16: 128 + (q & 127), less 128 or (q negative) 256.
-template <typename T>
-__device__ __forceinline__ void codes_to_16bit(uint32_t x, uint32_t& lo, uint32_t& hi) {
-  if constexpr (std::is_same<T, __half>::value) {
-    x ^= 0x80808080u;
-    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
-    __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), bias);
-    lo = *reinterpret_cast<uint32_t*>(&r);
-    r = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
-    hi = *reinterpret_cast<uint32_t*>(&r);
-  } else {
-    uint32_t y[2] = {__byte_perm(x, 0, 0x4140), __byte_perm(x, 0, 0x4342)};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t p = (y[i] & 0x007f007fu) | 0x43004300u, m = (y[i] & 0x00800080u) | 0x43004300u;
-      __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&p),
-                                 *reinterpret_cast<__nv_bfloat162*>(&m));
-      (i == 0 ? lo : hi) = *reinterpret_cast<uint32_t*>(&r);
-    }
-  }
-}
-
 // A [128 x D] code tile to a 16-bit tile of 128-byte-swizzled [128 x 64] boxes, by 128 threads:
 // 16 codes each per step. The lanes of columns 64-127 store their two chunks in the other order,
 // which keeps the eight lanes of a store phase on different banks.
 template <typename T, int D>
 __device__ __forceinline__ void convert_tile(const uint8_t* codes, uint8_t* tile, int tid) {
   constexpr int kChunks = D / 16;
-#pragma unroll 4
-  for (int i = 0; i < kChunks; ++i) {
-    const int at = i * 128 + tid;
-    const int row = at / kChunks, c = at % kChunks;
-    const uint4 x = *reinterpret_cast<const uint4*>(codes + at * 16);
-    uint4 y[2];
-    codes_to_16bit<T>(x.x, y[0].x, y[0].y);
-    codes_to_16bit<T>(x.y, y[0].z, y[0].w);
-    codes_to_16bit<T>(x.z, y[1].x, y[1].y);
-    codes_to_16bit<T>(x.w, y[1].z, y[1].w);
-    uint8_t* box = tile + (c >> 2) * kBoxBytes;
-    const int chunk = (2 * c) & 7;
-    const int swap = c >> 2;
-    *reinterpret_cast<uint4*>(box + sw128_offset(row, chunk + swap)) = swap ? y[1] : y[0];
-    *reinterpret_cast<uint4*>(box + sw128_offset(row, chunk + 1 - swap)) = swap ? y[0] : y[1];
+  constexpr int kBatch = 4;   // loads in flight: the compiler cannot move one past a store
+  const int c = tid % kChunks, swap = c >> 2;
+  const int row0 = tid / kChunks;
+  uint8_t* box = tile + (c >> 2) * kBoxBytes;
+#pragma unroll 1
+  for (int i0 = 0; i0 < kChunks; i0 += kBatch) {
+    uint4 x[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      x[i] = *reinterpret_cast<const uint4*>(codes + ((i0 + i) * 128 + tid) * 16);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      uint4 y0, y1;
+      codes_to_16bit<T>(x[i].x, y0.x, y0.y);
+      codes_to_16bit<T>(x[i].y, y0.z, y0.w);
+      codes_to_16bit<T>(x[i].z, y1.x, y1.y);
+      codes_to_16bit<T>(x[i].w, y1.z, y1.w);
+      const int row = row0 + (i0 + i) * (128 / kChunks), chunk = (2 * c) & 7;
+      *reinterpret_cast<uint4*>(box + sw128_offset(row, chunk + swap)) = swap ? y1 : y0;
+      *reinterpret_cast<uint4*>(box + sw128_offset(row, chunk + 1 - swap)) = swap ? y0 : y1;
+    }
   }
 }
 
@@ -452,16 +199,6 @@ __device__ __forceinline__ void exp_store(const float* sf, float sl2, float nref
   }
 }
 
-template <typename T>
-__device__ __forceinline__ uint4 pack8(const float* x, float scale) {
-  uint4 r;
-  r.x = pack2<T>(x[0] * scale, x[1] * scale);
-  r.y = pack2<T>(x[2] * scale, x[3] * scale);
-  r.z = pack2<T>(x[4] * scale, x[5] * scale);
-  r.w = pack2<T>(x[6] * scale, x[7] * scale);
-  return r;
-}
-
 // --------------------------------------------------------------------------------------------
 // The kernel
 // --------------------------------------------------------------------------------------------
@@ -473,14 +210,15 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   using G = Geometry<D, kInt8>;
   using P = typename std::conditional<kInt8, __half, T>::type;   // weights, and V as multiplied
-  using Sh = Shared<G::kSlots, G::kCodeSlots>;
-  constexpr int kSlots = G::kSlots;
+  using Sh = Shared<G::kKSlots, G::kVSlots, G::kCodeSlots>;
+  constexpr int kKSlots = G::kKSlots, kVSlots = G::kVSlots;
   constexpr int kTileBytes = G::kTileBytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* q_smem = smem;
-  uint8_t* ring = smem + G::kRingOffset;
+  uint8_t* k_ring = smem + G::kRingOffset;
+  uint8_t* v_ring = k_ring + kKSlots * kTileBytes;
   Sh* sh = reinterpret_cast<Sh*>(smem + G::kTailOffset);
 
   const int warp = threadIdx.x >> 5;
@@ -488,9 +226,13 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
 
   if (threadIdx.x == 0) {
     sh->abort_flag = 0;
-    for (int i = 0; i < kSlots; ++i) {
-      mbar_init(&sh->kv_full[i], kInt8 ? 128 : 1);
-      mbar_init(&sh->kv_empty[i], 1);
+    for (int i = 0; i < kKSlots; ++i) {
+      mbar_init(&sh->k_full[i], kInt8 ? 128 : 1);
+      mbar_init(&sh->k_empty[i], 1);
+    }
+    for (int i = 0; i < kVSlots; ++i) {
+      mbar_init(&sh->v_full[i], kInt8 ? 128 : 1);
+      mbar_init(&sh->v_empty[i], 1);
     }
     for (int i = 0; i < G::kCodeSlots; ++i) {
       mbar_init(&sh->code_full[i], 1);
@@ -520,8 +262,8 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     tmem_alloc(&sh->tmem_base, kTmemCols);
     tmem_relinquish();
   }
-  find_share(a, sh, reinterpret_cast<int64_t*>(ring));
-  fence_proxy_async_shared();   // the ring was written here; TMA writes it next
+  find_share(a, &sh->share, reinterpret_cast<int64_t*>(k_ring));
+  fence_proxy_async_shared();   // the rings were written here; TMA writes it next
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -534,9 +276,9 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
   if (warp == kProducerWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kOtherRegs));
     // ------------------------------- TMA producer -------------------------------
-    // Per segment: Q tile 0, K, Q tile 1, V, K, V, ... Lane i issues copy i of a tile (a part of
-    // box_rows cache rows and, at 16 bits, one of the column boxes) from the block it read one
-    // tile ahead.
+    // Per segment: Q tile 0, K 0, Q tile 1, K 1, V 0, K 2, V 1, ... Lane i issues copy i of a tile (a
+    // part of box_rows cache rows and, at 16 bits, one of the column boxes) from a block it read
+    // one tile ahead.
     constexpr int kCols = kInt8 ? 1 : G::kBoxes;
     const int parts = kBN / a.box_rows;
     const bool issues = lane < parts * kCols;
@@ -545,10 +287,44 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     const int page_size = a.cache.page_size;
     const int max_blocks = paged ? a.cache.max_seqlen / page_size : 0;
     const uint32_t q_bytes = static_cast<uint32_t>(a.group * a.tile_tokens * D * 2);
-    int issued = 0;              // K/V tiles issued
+    constexpr int kCodeSlots = kInt8 ? G::kCodeSlots : 1;
+    int k_issued = 0, v_issued = 0;   // tiles
     int q_loads[2] = {0, 0};
     bool ok = true;
-    walk.start(a, sh);
+    // Copies the tile at `tile` (this lane's part from block blk) to the next place of its ring.
+    auto load = [&](bool is_v, int tile, int blk) -> bool {
+      uint64_t *full, *empty;
+      uint8_t* dst;
+      int n, slots;
+      if constexpr (kInt8) {
+        n = k_issued + v_issued;
+        slots = kCodeSlots;
+        full = &sh->code_full[n % slots];
+        empty = &sh->code_empty[n % slots];
+        dst = smem + G::kCodeOffset + (n % slots) * G::kCodeBytes + part * a.box_rows * D;
+      } else {
+        n = is_v ? v_issued : k_issued;
+        slots = is_v ? kVSlots : kKSlots;
+        full = is_v ? &sh->v_full[n % slots] : &sh->k_full[n % slots];
+        empty = is_v ? &sh->v_empty[n % slots] : &sh->k_empty[n % slots];
+        dst = (is_v ? v_ring : k_ring) + (n % slots) * kTileBytes + col * kBoxBytes +
+              part * a.box_rows * 128;
+      }
+      bool free = n < slots || mbar_wait(empty, ((n / slots) - 1) & 1, guard);
+      if (!__all_sync(0xffffffffu, free)) return false;
+      if (lane == 0) mbar_arrive_expect_tx(full, kInt8 ? G::kCodeBytes : kTileBytes);
+      __syncwarp();
+      if (issues) {
+        const TmaCoords& c = is_v ? a.vc : a.kc;
+        const int key = tile * kBN + part * a.box_rows;
+        const int row = paged ? key % page_size : key;
+        tma_load_4d(dst, is_v ? &tmv : &tmk, full, col * 64, tma_c(c, 1, row, s.hkv, blk),
+                    tma_c(c, 2, row, s.hkv, blk), tma_c(c, 3, row, s.hkv, blk));
+      }
+      ++(is_v ? v_issued : k_issued);
+      return true;
+    };
+    walk.start(a, sh->share);
     while (ok && walk.next(a, s)) {
       if (s.tiles == 0) continue;
       const int32_t* table = a.cache.block_tables + s.b * a.cache.bt_stride;
@@ -570,80 +346,66 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
         ++q_loads[t];
         return true;
       };
-      int blk = block_of(s.t0);
-      ok = __all_sync(0xffffffffu, load_q(0));
+      int blk = block_of(s.t0), blk1 = s.t0 + 1 < s.t1 ? block_of(s.t0 + 1) : 0;
+      ok = __all_sync(0xffffffffu, load_q(0)) && load(false, s.t0, blk) &&
+           __all_sync(0xffffffffu, load_q(1));
       for (int tile = s.t0; ok && tile < s.t1; ++tile) {
-        const int next_blk = tile + 1 < s.t1 ? block_of(tile + 1) : 0;
-        const int key = tile * kBN + part * a.box_rows;
-        const int row = paged ? key % page_size : key;
-        for (int kind = 0; ok && kind < 2; ++kind) {
-          constexpr int kRing = kInt8 ? G::kCodeSlots : kSlots;
-          const int slot = issued % kRing;
-          uint64_t* empty = kInt8 ? &sh->code_empty[slot] : &sh->kv_empty[slot];
-          uint64_t* full = kInt8 ? &sh->code_full[slot] : &sh->kv_full[slot];
-          if (issued >= kRing) ok = mbar_wait(empty, ((issued / kRing) - 1) & 1, guard);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(full, kInt8 ? G::kCodeBytes : kTileBytes);
-          __syncwarp();
-          if (issues) {
-            const TmaCoords& c = kind == 0 ? a.kc : a.vc;
-            uint8_t* dst = kInt8 ? smem + G::kCodeOffset + slot * G::kCodeBytes + part * a.box_rows * D
-                                 : ring + slot * kTileBytes + col * kBoxBytes + part * a.box_rows * 128;
-            tma_load_4d(dst, kind == 0 ? &tmk : &tmv, full, col * 64, tma_c(c, 1, row, s.hkv, blk),
-                        tma_c(c, 2, row, s.hkv, blk), tma_c(c, 3, row, s.hkv, blk));
-          }
-          ++issued;
-          if (tile == s.t0 && kind == 0) ok = __all_sync(0xffffffffu, load_q(1));
-        }
-        blk = next_blk;
+        const int blk2 = tile + 2 < s.t1 ? block_of(tile + 2) : 0;
+        if (tile + 1 < s.t1) ok = load(false, tile + 1, blk1);
+        if (ok) ok = load(true, tile, blk);
+        blk = blk1;
+        blk1 = blk2;
       }
     }
     // Wait for the copies still landing before the CTA may exit.
     if (lane == 0) {
-      constexpr int kRing = kInt8 ? G::kCodeSlots : kSlots;
-      for (int t = 0; t < 2; ++t) {
-        if (q_loads[t] > 0) mbar_wait(&sh->q_full[t], (q_loads[t] - 1) & 1, guard);
-      }
-      for (int i = issued > kRing ? issued - kRing : 0; i < issued; ++i) {
-        uint64_t* full = kInt8 ? &sh->code_full[i % kRing] : &sh->kv_full[i % kRing];
-        if (!mbar_wait(full, (i / kRing) & 1, guard)) break;
+      auto drain = [&](uint64_t* full, int slots, int issued) {
+        for (int i = issued > slots ? issued - slots : 0; i < issued; ++i) {
+          if (!mbar_wait(full + i % slots, (i / slots) & 1, guard)) break;
+        }
+      };
+      drain(&sh->q_full[0], 1, q_loads[0]);
+      drain(&sh->q_full[1], 1, q_loads[1]);
+      if constexpr (kInt8) {
+        drain(sh->code_full, kCodeSlots, k_issued + v_issued);
+      } else {
+        drain(sh->k_full, kKSlots, k_issued);
+        drain(sh->v_full, kVSlots, v_issued);
       }
     }
   } else if (warp == kMmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kOtherRegs));
     // ------------------------------- MMA issuer -------------------------------
-    // The warp runs this loop together; one lane issues every tcgen05.mma and commit. Key tile i
-    // of a segment is ring entries 2 i (K) and 2 i + 1 (V). A one-tile item's second chain reads
-    // Q tile 0 as well.
+    // The warp runs this loop together; one lane issues every tcgen05.mma and commit. A one-tile
+    // item's second chain reads Q tile 0 as well.
     constexpr int kFmtQk = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
     constexpr int kFmtPv = std::is_same<P, __nv_bfloat16>::value ? 1 : 0;
     constexpr uint32_t kIdescQk = umma_idesc_f16(kFmtQk, kBM, kBN, 0);
     constexpr uint32_t kIdescPv = umma_idesc_f16(kFmtPv, kBM, D, 1);
     const bool leader = elect_one();
     const Desc q_desc(umma_smem_desc_sw128(smem_u32(q_smem), 16, 1024));
-    const Desc ring_k(umma_smem_desc_sw128(smem_u32(ring), 16, 1024));
-    const Desc ring_v(umma_smem_desc_sw128(smem_u32(ring), kBoxBytes, 1024));
+    const Desc ring_k(umma_smem_desc_sw128(smem_u32(k_ring), 16, 1024));
+    const Desc ring_v(umma_smem_desc_sw128(smem_u32(v_ring), kBoxBytes, 1024));
     auto commit = [&](uint64_t* bar) {
       if (leader) umma_commit(bar);
     };
-    int base = 0;                   // ring entry of the segment's first K tile
+    int base = 0;                   // key tiles of earlier segments
     int q_waits[2] = {0, 0}, p_waits[2] = {0, 0};
     bool ok = true, issued_any = false;
-    auto wait_ring = [&](int i) {
-      return __all_sync(0xffffffffu, mbar_wait(&sh->kv_full[i % kSlots], (i / kSlots) & 1, guard));
+    auto wait_tile = [&](uint64_t* full, int slots, int i) {
+      return __all_sync(0xffffffffu, mbar_wait(full + i % slots, (i / slots) & 1, guard));
     };
-    walk.start(a, sh);
+    walk.start(a, sh->share);
     while (ok && walk.next(a, s)) {
       if (s.tiles == 0) continue;
       issued_any = true;
       const int steps = max(s.count[0], s.count[1]);
       // Q K^T of chain c's step j; frees what its last reader is.
       auto issue_qk = [&](int c, int j) -> bool {
-        const int entry = base + 2 * s.place(c, j);
-        if (!wait_ring(entry)) return false;
+        const int entry = base + s.place(c, j);
+        if (!wait_tile(sh->k_full, kKSlots, entry)) return false;
         tc_fence_after();
-        const int slot = entry % kSlots;
+        const int slot = entry % kKSlots;
         const int q_tile = s.dual ? 0 : c;
         if (leader) {
           const Desc qd = q_desc.at(q_tile * kTileBytes);
@@ -654,7 +416,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
                     kIdescQk, kk > 0);
           umma_commit(&sh->s_full[c]);
         }
-        if (s.dual || c == 1) commit(&sh->kv_empty[slot]);
+        if (s.dual || c == 1) commit(&sh->k_empty[slot]);
         // The chain's last Q K^T (of both chains for a shared Q tile: the one issued last).
         if (s.dual ? s.place(c, j) + 1 == s.t1 - s.t0 : j + 1 == s.count[c])
           commit(&sh->q_free[q_tile]);
@@ -675,15 +437,15 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
         for (int c = 0; c < 2; ++c) {
           if (!ok) break;
           if (j < s.count[c]) {
-            const int entry = base + 2 * s.place(c, j) + 1;
-            const int slot = entry % kSlots;
-            ok = wait_ring(entry);
+            const int entry = base + s.place(c, j);
+            const int slot = entry % kVSlots;
+            ok = wait_tile(sh->v_full, kVSlots, entry);
             if (!ok) break;
             if constexpr (!kInt8) {
               const int keys = s.seq.len - s.tile(c, j) * kBN;   // of this tile
               if (keys < kBN && zeroed != entry) {
                 zeroed = entry;
-                uint8_t* v = ring + slot * kTileBytes;
+                uint8_t* v = v_ring + slot * kTileBytes;
                 for (int i = lane; i < (kBN - keys) * 8 * G::kBoxes; i += 32) {
                   const int row = keys + i / (8 * G::kBoxes), chunk = i % (8 * G::kBoxes);
                   *reinterpret_cast<uint4*>(v + (chunk >> 3) * kBoxBytes + row * 128 +
@@ -710,10 +472,10 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
             }
             if (!ok) break;
             ++p_waits[c];
-            if (s.dual) commit(&sh->kv_empty[slot]);
+            if (s.dual) commit(&sh->v_empty[slot]);
           }
           // A two-tile item's V is read last by chain 1, whose tiles are the segment's.
-          if (!s.dual && c == 1) commit(&sh->kv_empty[(base + 2 * j + 1) % kSlots]);
+          if (!s.dual && c == 1) commit(&sh->v_empty[(base + j) % kVSlots]);
           if (j + 1 < s.count[c]) {
             ok = issue_qk(c, j + 1);
           } else if (j + 1 == s.count[c]) {
@@ -721,7 +483,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
           }
         }
       }
-      base += 2 * (s.t1 - s.t0);
+      base += s.t1 - s.t0;
     }
     // Every MMA issued has completed before TMEM may be released.
     if (issued_any) {
@@ -745,7 +507,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     int segments = 0;
     int4 meta0 = make_int4(0, 0, 0, 0), meta1 = make_int4(0, 0, 0, 0);
     bool ok = true;
-    walk.start(a, sh);
+    walk.start(a, sh->share);
     while (ok && walk.next(a, s)) {
       const int first_segment = segments++ == 0;
       // This row's token, and whether it holds one.
@@ -959,15 +721,32 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
       // ------------------------------- code converters -------------------------------
       // Thread r also holds key r of the tile: its scales are read one tile ahead, its block two.
       // A tile's scales go to slot (tile % kScaleSlots) before its K tile is published. The slot is
-      // free: the ring entries before this K tile were refilled, so P V of the tile kScaleSlots
-      // earlier has run, which follows that tile's softmax.
+      // free: the V tile two before this K tile has been converted, so P V of the tile kVSlots
+      // earlier than that one has run, which follows its softmax (and kVSlots + 2 <= kScaleSlots).
       const int tid = threadIdx.x - kConvertWarp * 32;
       const bool paged = a.cache.block_tables != nullptr;
       const int page_size = a.cache.page_size;
       const int max_blocks = paged ? a.cache.max_seqlen / page_size : 0;
-      int done = 0;   // code tiles converted
+      static_assert(kVSlots + 2 <= kScaleSlots, "a tile's scales outlive its softmax");
+      int k_done = 0, v_done = 0;   // tiles converted
       bool ok = true;
-      walk.start(a, sh);
+      // The next code tile, once it and its place in the 16-bit ring are there.
+      auto ready = [&](bool is_v, const uint8_t*& codes, uint8_t*& dst) -> bool {
+        const int n = k_done + v_done, slot = n % G::kCodeSlots;
+        const int at = is_v ? v_done : k_done, slots = is_v ? kVSlots : kKSlots;
+        uint64_t* empty = is_v ? &sh->v_empty[at % slots] : &sh->k_empty[at % slots];
+        codes = smem + G::kCodeOffset + slot * G::kCodeBytes;
+        dst = (is_v ? v_ring : k_ring) + (at % slots) * kTileBytes;
+        return mbar_wait(&sh->code_full[slot], (n / G::kCodeSlots) & 1, guard) &&
+               (at < slots || mbar_wait(empty, ((at / slots) - 1) & 1, guard));
+      };
+      auto publish = [&](bool is_v) {
+        fence_proxy_async_shared();
+        mbar_arrive(is_v ? &sh->v_full[v_done % kVSlots] : &sh->k_full[k_done % kKSlots]);
+        mbar_arrive(&sh->code_empty[(k_done + v_done) % G::kCodeSlots]);
+        ++(is_v ? v_done : k_done);
+      };
+      walk.start(a, sh->share);
       while (ok && walk.next(a, s)) {
         if (s.tiles == 0) continue;
         const int32_t* table = a.cache.block_tables + s.b * a.cache.bt_stride;
@@ -989,68 +768,48 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
                             s.hkv * a.cache.vs_stride[2]];
           }
         };
-        float sk, sv, sk_next = 0.f, sv_next = 0.f;
+        float sk, sv;
         scales_of(s.t0, block_of(s.t0), sk, sv);
         int blk_next = block_of(s.t0 + 1);
-        for (int tile = s.t0; ok && tile < s.t1; ++tile) {
-          if (tile + 1 < s.t1) {
-            scales_of(tile + 1, blk_next, sk_next, sv_next);
-            blk_next = block_of(tile + 2);
-          }
-          for (int kind = 0; ok && kind < 2; ++kind) {
-            const int code_slot = done % G::kCodeSlots, slot = done % kSlots;
-            ok = mbar_wait(&sh->code_full[code_slot], (done / G::kCodeSlots) & 1, guard) &&
-                 (done < kSlots || mbar_wait(&sh->kv_empty[slot], ((done / kSlots) - 1) & 1, guard));
-            if (!ok) break;
-            const uint8_t* codes = smem + G::kCodeOffset + code_slot * G::kCodeBytes;
-            uint8_t* dst = ring + slot * kTileBytes;
-            if (kind == 0) {
-              float* out = reinterpret_cast<float*>(smem + G::kScaleOffset) +
-                           ((done / 2) % kScaleSlots) * 3 * kBN + tid;
-              // Keys past the length have no weight. A scale that is not finite makes z, and so the
-              // weight, not finite for the rows that see the key, and adds nothing to others' sums.
-              const bool in = tile * kBN + tid < s.seq.len;
-              sv = sv < kMinScale ? kMinScale : sv;
-              out[0] = in ? sk * a.scale_log2 : 0.f;
-              out[kBN] = in ? __log2f(sv) : -INFINITY;
-              out[2 * kBN] = in && sv <= 0x1p+127f ? 1.f / sv : 0.f;
-              mbar_arrive(&sh->scale_full[(done / 2) % kScaleSlots]);
-              convert_tile<T, D>(codes, dst, tid);
-            } else {
-              convert_tile<__half, D>(codes, dst, tid);
+        for (int i = s.t0; ok && i <= s.t1; ++i) {   // K tile i, V tile i - 1
+          const uint8_t* codes;
+          uint8_t* dst;
+          if (i < s.t1) {
+            float sk_next = 0.f, sv_next = 0.f;
+            if (i + 1 < s.t1) {
+              scales_of(i + 1, blk_next, sk_next, sv_next);
+              blk_next = block_of(i + 2);
             }
-            fence_proxy_async_shared();
-            mbar_arrive(&sh->kv_full[slot]);
-            mbar_arrive(&sh->code_empty[code_slot]);
-            ++done;
+            ok = ready(false, codes, dst);
+            if (!ok) break;
+            // Keys past the length have no weight. A scale that is not finite makes z, and so the
+            // weight, not finite for the rows that see the key, and adds nothing to others' sums.
+            float* out = reinterpret_cast<float*>(smem + G::kScaleOffset) +
+                         (k_done % kScaleSlots) * 3 * kBN + tid;
+            const bool in = i * kBN + tid < s.seq.len;
+            sv = sv < kMinScale ? kMinScale : sv;
+            out[0] = in ? sk * a.scale_log2 : 0.f;
+            out[kBN] = in ? __log2f(sv) : -INFINITY;
+            out[2 * kBN] = in && sv <= 0x1p+127f ? 1.f / sv : 0.f;
+            mbar_arrive(&sh->scale_full[k_done % kScaleSlots]);
+            convert_tile<T, D>(codes, dst, tid);
+            publish(false);
+            sk = sk_next;
+            sv = sv_next;
           }
-          sk = sk_next;
-          sv = sv_next;
+          if (i > s.t0) {
+            ok = ready(true, codes, dst);
+            if (!ok) break;
+            convert_tile<__half, D>(codes, dst, tid);
+            publish(true);
+          }
         }
       }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kOtherRegs));
     // ------------------------------- warps 10 and 11 -------------------------------
-    // Rows of no sequence (before the first offset, behind the last) give 0 and -inf.
-    const Ragged& r = a.ragged;
-    int begin = 0, end = 0;
-    if (r.cu != nullptr) {
-      begin = min(max(__ldg(r.cu), 0), r.rows);
-      end = min(max(__ldg(r.cu + r.batch), begin), r.rows);
-    } else {
-      end = static_cast<int>(min(static_cast<int64_t>(r.batch) * r.rows_per_seq,
-                                 static_cast<int64_t>(r.rows)));
-    }
-    const int64_t missing = static_cast<int64_t>(begin + r.rows - end) * a.heads;
-    for (int64_t i = blockIdx.x * 2 + warp - 10; i < missing; i += gridDim.x * 2) {
-      const int64_t at = i / a.heads;
-      const int head = static_cast<int>(i - at * a.heads);
-      const int64_t out_row = at < begin ? at : end + (at - begin);
-      T* orow = static_cast<T*>(a.o) + out_row * a.o_stride[0] + head * a.o_stride[1];
-      if (lane < D / 8) reinterpret_cast<uint4*>(orow)[lane] = make_uint4(0, 0, 0, 0);
-      if (lane == 0) a.lse[out_row * a.heads + head] = -INFINITY;
-    }
+    zero_other_rows<T, D>(a, blockIdx.x * 2 + warp - 10, gridDim.x * 2, lane);
   }
 
   tc_fence_before();
@@ -1162,7 +921,7 @@ template <typename T, int D, bool kInt8>
 int launch(const ExtendArgs& a, const CUtensorMap& tmq, const CUtensorMap& tmk,
            const CUtensorMap& tmv, int ctas, int dev, cudaStream_t stream) {
   using G = Geometry<D, kInt8>;
-  constexpr int kSmem = G::kTailOffset + static_cast<int>(sizeof(Shared<G::kSlots, G::kCodeSlots>)) +
+  constexpr int kSmem = G::kTailOffset + static_cast<int>(sizeof(Shared<G::kKSlots, G::kVSlots, G::kCodeSlots>)) +
                         1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
   auto kernel = extend_kernel<T, D, kInt8>;
@@ -1182,7 +941,11 @@ int launch(const ExtendArgs& a, const CUtensorMap& tmq, const CUtensorMap& tmk,
     configured_device = dev;
   }
   kernel<<<ctas, G::kThreads, kSmem, stream>>>(a, tmq, tmk, tmv);
-  if (int st = check_cuda(cudaGetLastError(), "extend_kernel launch")) return st;
+  return check_cuda(cudaGetLastError(), "extend_kernel launch");
+}
+
+template <typename T, int D>
+int launch_merge(const ExtendArgs& a, int ctas, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, (a.part_rows * (D / 8) + 255) / 256);
   cfg.blockDim = dim3(256);
@@ -1194,6 +957,12 @@ int launch(const ExtendArgs& a, const CUtensorMap& tmq, const CUtensorMap& tmk,
   cfg.numAttrs = 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, extend_merge_kernel<T, D>, a, ctas),
                     "extend_merge_kernel launch");
+}
+
+template <typename T>
+int launch_merge_t(int head_dim, const ExtendArgs& a, int ctas, cudaStream_t stream) {
+  return head_dim == 128 ? launch_merge<T, 128>(a, ctas, stream)
+                         : launch_merge<T, 64>(a, ctas, stream);
 }
 
 template <typename T>
@@ -1258,15 +1027,38 @@ int validate(const flb_kv_cache* c, const flb_extend_params* p) {
 
 using namespace flb;
 
+namespace {
+
+// The partials of one launch: metadata, (m, l), O.
+size_t partial_bytes(size_t ctas, size_t rows, size_t head_dim) {
+  return align256(2 * ctas * sizeof(int4)) + align256(2 * ctas * rows * 2 * sizeof(float)) +
+         align256(2 * ctas * rows * head_dim * sizeof(float));
+}
+
+void set_partials(ExtendArgs* a, char* ws, size_t ctas, int rows) {
+  a->part_rows = rows;
+  a->part_meta = reinterpret_cast<int4*>(ws);
+  ws += align256(2 * ctas * sizeof(int4));
+  a->part_ml = reinterpret_cast<float*>(ws);
+  ws += align256(2 * ctas * static_cast<size_t>(rows) * 2 * sizeof(float));
+  a->part_o = reinterpret_cast<float*>(ws);
+}
+
+// Cache rows of one TMA box: whole tiles of a contiguous cache, else rows that never cross a page.
+int box_rows_for(const flb_kv_cache* c) {
+  return c->block_tables == nullptr || c->page_size % kBN == 0 ? kBN : std::min(c->page_size, 64);
+}
+
+}  // namespace
+
 extern "C" size_t flb_extend_workspace_bytes(int32_t rows, int32_t heads, int32_t heads_kv,
                                              int32_t head_dim, int32_t sm_count) {
   if (rows <= 0 || heads <= 0 || heads_kv <= 0 || heads % heads_kv != 0 ||
       heads / heads_kv > kBM || head_dim <= 0 || sm_count <= 0)
     return 0;
-  const size_t slots = 2 * static_cast<size_t>(sm_count);
-  const size_t part = static_cast<size_t>(part_rows(rows, heads / heads_kv));
-  return align256(slots * sizeof(int4)) + align256(slots * part * 2 * sizeof(float)) +
-         slots * part * head_dim * sizeof(float);
+  // Both kernels of a call over an int8 cache have partials of their own.
+  return partial_bytes(sm_count, kFewTile, head_dim) +
+         partial_bytes(sm_count, part_rows(rows, heads / heads_kv), head_dim);
 }
 
 extern "C" int flb_extend_fwd(const flb_kv_cache* c, const flb_extend_params* p,
@@ -1295,28 +1087,42 @@ extern "C" int flb_extend_fwd(const flb_kv_cache* c, const flb_extend_params* p,
   a.heads = p->heads;
   a.group = p->heads / c->heads_kv;
   a.causal = p->causal ? 1 : 0;
-  a.tile_tokens = kBM / a.group;
   a.scale_log2 = static_cast<float>(static_cast<double>(p->softmax_scale) * 1.4426950408889634);
   a.cache = kv_view(c);
-  const size_t slots = 2 * static_cast<size_t>(sm_count);
-  a.part_rows = part_rows(p->rows, a.group);
+  a.box_rows = box_rows_for(c);
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   char* ws = static_cast<char*>(p->workspace);
-  a.part_meta = reinterpret_cast<int4*>(ws);
-  ws += align256(slots * sizeof(int4));
-  a.part_ml = reinterpret_cast<float*>(ws);
-  ws += align256(slots * static_cast<size_t>(a.part_rows) * 2 * sizeof(float));
-  a.part_o = reinterpret_cast<float*>(ws);
+  auto merge = [&](const ExtendArgs& args) {
+    return p->dtype == FLB_BF16 ? launch_merge_t<__nv_bfloat16>(c->head_dim, args, sm_count, stream)
+                                : launch_merge_t<__half>(c->head_dim, args, sm_count, stream);
+  };
 
-  // Boxes of the cache: whole tiles of a contiguous cache, else rows that never cross a page.
-  const int ps = c->page_size;
-  a.box_rows = c->block_tables == nullptr || ps % kBN == 0 ? kBN : std::min(ps, 64);
+  // Which kernel: by the rows of every sequence when they are known here, else both (int8).
+  const bool int8 = c->dtype == FLB_INT8;
+  const bool known = p->cu_seqlens == nullptr || c->batch == 1;
+  const int64_t per_seq = p->cu_seqlens == nullptr ? p->rows_per_seq : p->rows;
+  const bool few = int8 && a.group <= kFewTile && (!known || per_seq <= kFewTile / a.group);
+  const bool many = !few || !known;
+  if (few) {
+    ExtendArgs f = a;
+    f.tile_tokens = kFewTile / a.group;
+    f.select = many ? kFewRows : kAllRows;
+    set_partials(&f, ws, sm_count, kFewTile);
+    if (int st = launch_extend_few(f, c, p->q, p->q_row_stride, p->q_head_stride, p->dtype,
+                                   sm_count, dev, stream))
+      return st;
+    if (int st = merge(f)) return st;
+  }
+  if (!many) return FLB_OK;
+  a.tile_tokens = kBM / a.group;
+  a.select = few ? kManyRows : kAllRows;
+  set_partials(&a, ws + partial_bytes(sm_count, kFewTile, c->head_dim), sm_count,
+               part_rows(p->rows, a.group));
   CUtensorMap tmq, tmk, tmv;
   const View4 kv = kv_view4(c, false), vv = kv_view4(c, true);
-  if (c->dtype == FLB_INT8) {
-    if (int st = encode_rows_map(&tmk, &a.kc, kv, a.box_rows, c->head_dim, FLB_INT8, false))
-      return st;
-    if (int st = encode_rows_map(&tmv, &a.vc, vv, a.box_rows, c->head_dim, FLB_INT8, false))
-      return st;
+  if (int8) {
+    if (int st = encode_rows_map(&tmk, &a.kc, kv, a.box_rows, c->head_dim, FLB_INT8, 0)) return st;
+    if (int st = encode_rows_map(&tmv, &a.vc, vv, a.box_rows, c->head_dim, FLB_INT8, 0)) return st;
   } else {
     if (int st = encode_rows_x64_map(&tmk, &a.kc, kv, a.box_rows, c->dtype)) return st;
     if (int st = encode_rows_x64_map(&tmv, &a.vc, vv, a.box_rows, c->dtype)) return st;
@@ -1324,8 +1130,8 @@ extern "C" int flb_extend_fwd(const flb_kv_cache* c, const flb_extend_params* p,
   if (int st = encode_group_map(&tmq, p->q, p->rows, c->heads_kv, a.group, c->head_dim,
                                 p->q_row_stride, p->q_head_stride, a.tile_tokens, p->dtype))
     return st;
-  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  if (p->dtype == FLB_BF16)
-    return launch_t<__nv_bfloat16>(c, a, tmq, tmk, tmv, sm_count, dev, stream);
-  return launch_t<__half>(c, a, tmq, tmk, tmv, sm_count, dev, stream);
+  const int st = p->dtype == FLB_BF16
+                     ? launch_t<__nv_bfloat16>(c, a, tmq, tmk, tmv, sm_count, dev, stream)
+                     : launch_t<__half>(c, a, tmq, tmk, tmv, sm_count, dev, stream);
+  return st != FLB_OK ? st : merge(a);
 }

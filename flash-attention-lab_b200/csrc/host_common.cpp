@@ -100,11 +100,11 @@ bool rows_16b_aligned(const View4& v) {
 
 int encode_rows_x64_map(CUtensorMap* map, TmaCoords* coords, const View4& v, int box_rows,
                         int dtype) {
-  return encode_rows_map(map, coords, v, box_rows, 64, dtype, true);
+  return encode_rows_map(map, coords, v, box_rows, 64, dtype, 128);
 }
 
 int encode_rows_map(CUtensorMap* map, TmaCoords* coords, const View4& v, int box_rows,
-                    int box_cols, int dtype, bool swizzle128) {
+                    int box_cols, int dtype, int swizzle) {
   if (!rows_16b_aligned(v)) {
     return fail(FLB_ERR_MISALIGNED,
                 "tensor must have 16-byte aligned rows (data pointer and strides)");
@@ -165,7 +165,9 @@ int encode_rows_map(CUtensorMap* map, TmaCoords* coords, const View4& v, int box
                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUresult r = encode(map, type, 4, const_cast<void*>(v.base), dims, strides, box, elem_strides,
                       CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                      swizzle == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                     : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                     : CU_TENSOR_MAP_SWIZZLE_NONE,
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     return fail(FLB_ERR_CUDA,

@@ -41,11 +41,11 @@ struct TmaCoords {
 int encode_rows_x64_map(CUtensorMap* map, TmaCoords* coords, const View4& v, int box_rows,
                         int dtype);
 
-// The general form: a [box_rows along S] x [box_cols along D] box, 128-byte swizzled or not
-// (box_cols * element size must be a multiple of 16 bytes; 64 columns of 16-bit elements when
-// swizzled).
+// The general form: a [box_rows along S] x [box_cols along D] box, swizzled over `swizzle` bytes
+// (128, 64, or 0 for none; box_cols * element size must be a multiple of 16 bytes, and equal to
+// `swizzle` when swizzled).
 int encode_rows_map(CUtensorMap* map, TmaCoords* coords, const View4& v, int box_rows,
-                    int box_cols, int dtype, bool swizzle128);
+                    int box_cols, int dtype, int swizzle);
 
 // A 5-D map over a 16-bit `v` with head_dim 128 whose box moves a whole [box_rows x 128] tile in
 // one copy: dimensions [64 columns] x [S] x [2 column halves, stride 128 bytes] x [H, B ordered
