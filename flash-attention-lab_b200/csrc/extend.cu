@@ -284,8 +284,6 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     const bool issues = lane < parts * kCols;
     const int part = lane / kCols, col = lane % kCols;
     const bool paged = a.cache.block_tables != nullptr;
-    const int page_size = a.cache.page_size;
-    const int max_blocks = paged ? a.cache.max_seqlen / page_size : 0;
     const uint32_t q_bytes = static_cast<uint32_t>(a.group * a.tile_tokens * D * 2);
     constexpr int kCodeSlots = kInt8 ? G::kCodeSlots : 1;
     int k_issued = 0, v_issued = 0;   // tiles
@@ -317,7 +315,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
       if (issues) {
         const TmaCoords& c = is_v ? a.vc : a.kc;
         const int key = tile * kBN + part * a.box_rows;
-        const int row = paged ? key % page_size : key;
+        const int row = paged ? key - a.cache.page.div(key) * a.cache.page.d : key;
         tma_load_4d(dst, is_v ? &tmv : &tmk, full, col * 64, tma_c(c, 1, row, s.hkv, blk),
                     tma_c(c, 2, row, s.hkv, blk), tma_c(c, 3, row, s.hkv, blk));
       }
@@ -330,8 +328,8 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
       const int32_t* table = a.cache.block_tables + s.b * a.cache.bt_stride;
       auto block_of = [&](int tile) -> int {
         if (!paged) return s.b;
-        const int page = (tile * kBN + part * a.box_rows) / page_size;
-        const int blk = issues && page < max_blocks ? __ldg(table + page) : -1;
+        const int page = a.cache.page.div(tile * kBN + part * a.box_rows);
+        const int blk = issues && page < a.cache.max_blocks ? __ldg(table + page) : -1;
         return blk >= 0 && blk < a.cache.num_blocks ? blk : -1;   // -1 reads as zeros
       };
       auto load_q = [&](int t) -> bool {
@@ -725,8 +723,6 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
       // earlier than that one has run, which follows its softmax (and kVSlots + 2 <= kScaleSlots).
       const int tid = threadIdx.x - kConvertWarp * 32;
       const bool paged = a.cache.block_tables != nullptr;
-      const int page_size = a.cache.page_size;
-      const int max_blocks = paged ? a.cache.max_seqlen / page_size : 0;
       static_assert(kVSlots + 2 <= kScaleSlots, "a tile's scales outlive its softmax");
       int k_done = 0, v_done = 0;   // tiles converted
       bool ok = true;
@@ -752,8 +748,8 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
         const int32_t* table = a.cache.block_tables + s.b * a.cache.bt_stride;
         auto block_of = [&](int tile) -> int {
           if (!paged) return s.b;
-          const int page = (tile * kBN + tid) / page_size;
-          const int blk = page < max_blocks ? __ldg(table + page) : -1;
+          const int page = a.cache.page.div(tile * kBN + tid);
+          const int blk = page < a.cache.max_blocks ? __ldg(table + page) : -1;
           return blk < a.cache.num_blocks ? blk : -1;
         };
         auto scales_of = [&](int tile, int blk, float& sk, float& sv) {
@@ -761,7 +757,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
           sk = 0.f;
           sv = kMinScale;
           if (key < s.seq.len && blk >= 0) {
-            const int64_t r = paged ? key % page_size : key;
+            const int64_t r = paged ? key - a.cache.page.div(key) * a.cache.page.d : key;
             sk = a.cache.ks[blk * a.cache.ks_stride[0] + r * a.cache.ks_stride[1] +
                             s.hkv * a.cache.ks_stride[2]];
             sv = a.cache.vs[blk * a.cache.vs_stride[0] + r * a.cache.vs_stride[1] +

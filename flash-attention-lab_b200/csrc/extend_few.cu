@@ -4,10 +4,12 @@
 // memory straight into the registers of 16 x 8 x 16 warp MMAs instead of through 16-bit tiles (the
 // tcgen05 form of extend.cu took 297 us for 8 sequences of 24K keys, H_kv 8, D 128).
 //
-//  * One CTA per SM: a producer warp streams [128 keys x D] tiles of K and V codes by TMA, with the
-//    keys' scales by 4-byte cp.async into the same ring stage, and eight consumer warps take 16 keys of
-//    every tile, each with its own online softmax; their results are joined in a fixed order at
-//    the end of a segment.
+//  * One CTA per SM: one warp streams [128 keys x D] tiles of K and V codes by TMA, another turns the
+//    keys' scales into what the scores need (below) beside them in the ring stage, and eight
+//    consumer warps take 16 keys of every tile, each with its own online softmax; their results
+//    are joined in a fixed order at the end of a segment. Block tables are read 32 entries at a
+//    time. (One producer warp for copies and scales, with a table load per key, bounded 16-row
+//    pages: 5000 clocks per tile where the consumers took 2400.)
 //  * Q is the A operand (rows = tokens x heads), in fp16: bf16 queries are scaled to [1, 2) of
 //    their row's maximum by a power of two, which is exact down to 2^-17 of the maximum and off by at
 //    most 2^-25 of it below. The order of a dot product is free, so thread t of a quad takes D / 4
@@ -24,7 +26,9 @@ namespace flb {
 namespace {
 
 constexpr int kWarps = 8;             // consumers: 16 keys of a tile each
-constexpr int kFewThreads = (kWarps + 1) * 32;
+constexpr int kCopyWarp = kWarps;      // TMA of the codes
+constexpr int kScaleWarp = kWarps + 1;
+constexpr int kFewThreads = (kWarps + 2) * 32;
 static_assert(kWarps * 16 == kBN, "the consumers cover a tile");
 
 template <int D>
@@ -32,7 +36,7 @@ struct FewGeometry {
   static constexpr int kTileBytes = kBN * D;          // K or V codes
   static constexpr int kStages = D == 128 ? 4 : 8;    // 128 KB of codes
   static constexpr int kScaleOffset = kStages * 2 * kTileBytes;
-  static constexpr int kScaleBytes = 2 * kBN * 4;     // sk, sv of one stage
+  static constexpr int kScaleBytes = 3 * kBN * 4;     // sk, log2 sv and 1 / sv of one stage
   static constexpr int kJoinOffset = kScaleOffset + kStages * kScaleBytes;
   static constexpr int kJoinBytes = kWarps * kFewTile * (D + 2) * 4;
   static constexpr int kTailOffset = kJoinOffset + kJoinBytes;
@@ -47,16 +51,48 @@ struct FewShared {
   Share share;
 };
 
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const float* src, bool valid) {
-  const int bytes = valid ? 4 : 0;   // 0: the destination is zeroed
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-               : "memory");
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
+// The block table of one sequence as a warp reads it: 32 entries from `base` and the 32 after
+// them, one per lane, the second half a window ahead. Pages are asked for in tile order; a tile's
+// lie in [base, base + 64) once advance() was called with its first one.
+struct BlockWindow {
+  const int32_t* table;
+  int base, cur, next;
+
+  __device__ __forceinline__ int entry(const KvView& c, int page) const {
+    const int blk = page < c.max_blocks ? __ldg(table + page) : -1;
+    return blk >= 0 && blk < c.num_blocks ? blk : -1;   // -1 reads as zeros
+  }
+  __device__ __forceinline__ void start(const KvView& c, int b, int first_page, int lane) {
+    table = c.block_tables + b * c.bt_stride;
+    base = first_page;
+    cur = entry(c, base + lane);
+    next = entry(c, base + 32 + lane);
+  }
+  __device__ __forceinline__ void advance(const KvView& c, int first_page, int lane) {
+    if (first_page >= base + 32) {
+      base += 32;
+      cur = next;
+      next = entry(c, base + 32 + lane);
+    }
+  }
+  __device__ __forceinline__ int at(int page) const {   // every lane calls this
+    const int i = page - base;
+    const int lo = __shfl_sync(0xffffffffu, cur, i & 31);
+    const int hi = __shfl_sync(0xffffffffu, next, i & 31);
+    return i < 32 ? lo : hi;
+  }
+};
 
 // Byte offset of 16-byte chunk c of row r in a code tile as TMA wrote it (128- or 64-byte swizzle).
 template <int D>
@@ -114,12 +150,12 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   if (threadIdx.x == 0) {
     sh->abort_flag = 0;
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&sh->full[i], 33);   // the TMA bytes and each producer lane's scales
+      mbar_init(&sh->full[i], 33);   // the TMA bytes and each lane's scales
       mbar_init(&sh->empty[i], kWarps);
     }
     fence_barrier_init();
   }
-  if (warp == kWarps && lane == 0) {
+  if (warp == kCopyWarp && lane == 0) {
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
   }
@@ -131,37 +167,29 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   Segment s;
   walk.start(a, sh->share);
 
-  if (warp == kWarps) {
-    // ------------------------------- producer -------------------------------
-    // Lane i issues copy i of a tile (a part of box_rows rows, of K or of V) and the scales of
-    // keys i, i + 32, i + 64, i + 96. Block ids are read one tile ahead.
+  if (warp == kCopyWarp) {
+    // ------------------------------- copies -------------------------------
+    // Lane i issues copy i of a tile: a part of box_rows rows, of K or of V.
     const int parts = kBN / a.box_rows;
     const bool issues = lane < 2 * parts;
     const bool is_v = lane >= parts;
-    const int part = is_v ? lane - parts : lane;
+    const int offset = (is_v ? lane - parts : lane) % parts * a.box_rows;   // of the part's keys
     const bool paged = a.cache.block_tables != nullptr;
-    const int page_size = a.cache.page_size;
-    const int max_blocks = paged ? a.cache.max_seqlen / page_size : 0;
+    const CUtensorMap* map = is_v ? &tmv : &tmk;
+    const TmaCoords& c = is_v ? a.vc : a.kc;
+    BlockWindow window;
     int issued = 0;
     bool ok = true;
     while (ok && walk.next(a, s)) {
-      const int32_t* table = a.cache.block_tables + s.b * a.cache.bt_stride;
-      auto block_of = [&](int key) -> int {
-        if (!paged) return s.b;
-        const int page = key / page_size;
-        const int blk = page < max_blocks ? __ldg(table + page) : -1;
-        return blk >= 0 && blk < a.cache.num_blocks ? blk : -1;   // -1 reads as zeros
-      };
-      int blk = block_of(s.t0 * kBN + part * a.box_rows), key_blk[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) key_blk[i] = block_of(s.t0 * kBN + lane + 32 * i);
+      if (paged) window.start(a.cache, s.b, a.cache.page.div(s.t0 * kBN), lane);
       for (int tile = s.t0; tile < s.t1; ++tile) {
-        const int k0 = tile * kBN;
-        int next_blk = 0, next_key_blk[4] = {0, 0, 0, 0};
-        if (tile + 1 < s.t1) {
-          next_blk = block_of(k0 + kBN + part * a.box_rows);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) next_key_blk[i] = block_of(k0 + kBN + lane + 32 * i);
+        const int key = tile * kBN + offset;
+        int blk = s.b, row = key;
+        if (paged) {
+          const int page = a.cache.page.div(key);
+          window.advance(a.cache, __shfl_sync(0xffffffffu, page, 0), lane);
+          blk = window.at(page);
+          row = key - page * a.cache.page.d;
         }
         const int st = issued % kStages;
         ok = issued < kStages || mbar_wait(&sh->empty[st], ((issued / kStages) - 1) & 1, guard);
@@ -169,37 +197,87 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&sh->full[st], 2 * G::kTileBytes);
         __syncwarp();
-        if (issues) {
-          const TmaCoords& c = is_v ? a.vc : a.kc;
-          const int key = k0 + part * a.box_rows;
-          const int row = paged ? key % page_size : key;
-          uint8_t* dst = smem + (2 * st + (is_v ? 1 : 0)) * G::kTileBytes + part * a.box_rows * D;
-          tma_load_4d(dst, is_v ? &tmv : &tmk, &sh->full[st], 0, tma_c(c, 1, row, s.hkv, blk),
-                      tma_c(c, 2, row, s.hkv, blk), tma_c(c, 3, row, s.hkv, blk));
-        }
-        const uint32_t scales = smem_u32(smem + G::kScaleOffset + st * G::kScaleBytes);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = k0 + lane + 32 * i;
-          const bool in = key < s.seq.len && key_blk[i] >= 0;
-          const int64_t outer = in ? key_blk[i] : 0, row = !in ? 0 : paged ? key % page_size : key;
-          cp_async_4(scales + (lane + 32 * i) * 4,
-                     a.cache.ks + outer * a.cache.ks_stride[0] + row * a.cache.ks_stride[1] +
-                         s.hkv * a.cache.ks_stride[2], in);
-          cp_async_4(scales + (kBN + lane + 32 * i) * 4,
-                     a.cache.vs + outer * a.cache.vs_stride[0] + row * a.cache.vs_stride[1] +
-                         s.hkv * a.cache.vs_stride[2], in);
-        }
-        cp_async_arrive(&sh->full[st]);
+        if (issues)
+          tma_load_4d(smem + (2 * st + (is_v ? 1 : 0)) * G::kTileBytes + offset * D, map,
+                      &sh->full[st], 0, tma_c(c, 1, row, s.hkv, blk), tma_c(c, 2, row, s.hkv, blk),
+                      tma_c(c, 3, row, s.hkv, blk));
         ++issued;
-        blk = next_blk;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) key_blk[i] = next_key_blk[i];
       }
     }
     // Wait for the copies still landing before the CTA may exit.
     for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
       if (!mbar_wait(&sh->full[i % kStages], (i / kStages) & 1, guard)) break;
+    }
+    return;
+  }
+  if (warp == kScaleWarp) {
+    // ------------------------------- scales -------------------------------
+    // Lane i turns the scales of keys 4 i .. 4 i + 3 of a tile, read one tile ahead, into sk,
+    // log2 sv and 1 / sv. They lie in one page. With a.wide_scales they are 16 contiguous bytes.
+    const bool paged = a.cache.block_tables != nullptr;
+    const int64_t ks_row = a.cache.ks_stride[1], vs_row = a.cache.vs_stride[1];
+    BlockWindow window;
+    int issued = 0;
+    bool ok = true;
+    while (ok && walk.next(a, s)) {
+      if (paged) window.start(a.cache, s.b, a.cache.page.div(s.t0 * kBN), lane);
+      // Keys past the length are not read: they stay hidden, whatever their scales.
+      auto fetch = [&](int tile, float (&sk)[4], float (&sv)[4]) {
+        const int key = tile * kBN + 4 * lane;
+        int64_t outer = s.b, row = key;
+        if (paged) {
+          const int page = a.cache.page.div(key);
+          window.advance(a.cache, __shfl_sync(0xffffffffu, page, 0), lane);
+          outer = window.at(page);
+          row = key - page * a.cache.page.d;
+        }
+        const int keys = outer >= 0 ? s.seq.len - key : 0;
+        const float* k = a.cache.ks + outer * a.cache.ks_stride[0] + row * ks_row +
+                         s.hkv * a.cache.ks_stride[2];
+        const float* v = a.cache.vs + outer * a.cache.vs_stride[0] + row * vs_row +
+                         s.hkv * a.cache.vs_stride[2];
+        if (a.wide_scales && keys >= 4) {
+          const float4 x = __ldg(reinterpret_cast<const float4*>(k));
+          const float4 y = __ldg(reinterpret_cast<const float4*>(v));
+          sk[0] = x.x, sk[1] = x.y, sk[2] = x.z, sk[3] = x.w;
+          sv[0] = y.x, sv[1] = y.y, sv[2] = y.z, sv[3] = y.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sk[i] = i < keys ? __ldg(k + i * ks_row) : 0.f;
+            sv[i] = i < keys ? __ldg(v + i * vs_row) : kMinScale;
+          }
+        }
+      };
+      float sk[4], sv[4];
+      if (s.t0 < s.t1) fetch(s.t0, sk, sv);
+      for (int tile = s.t0; tile < s.t1; ++tile) {
+        float sk_next[4] = {0.f, 0.f, 0.f, 0.f}, sv_next[4] = {0.f, 0.f, 0.f, 0.f};
+        if (tile + 1 < s.t1) fetch(tile + 1, sk_next, sv_next);
+        const int st = issued % kStages;
+        ok = issued < kStages || mbar_wait(&sh->empty[st], ((issued / kStages) - 1) & 1, guard);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        float add[4], inv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = sv[i] < kMinScale ? kMinScale : sv[i];
+          add[i] = lg2(v);
+          // A scale that is not finite reaches the rows that see its key through z only.
+          inv[i] = v <= 0x1p+127f ? rcp(v) : 0.f;
+        }
+        float4* dst = reinterpret_cast<float4*>(smem + G::kScaleOffset + st * G::kScaleBytes) + lane;
+        dst[0] = make_float4(sk[0], sk[1], sk[2], sk[3]);
+        dst[kBN / 4] = make_float4(add[0], add[1], add[2], add[3]);
+        dst[2 * (kBN / 4)] = make_float4(inv[0], inv[1], inv[2], inv[3]);
+        mbar_arrive(&sh->full[st]);
+        ++issued;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sk[i] = sk_next[i];
+          sv[i] = sv_next[i];
+        }
+      }
     }
     zero_other_rows<T, D>(a, blockIdx.x, gridDim.x, lane);
     return;
@@ -283,7 +361,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                                                            st * G::kScaleBytes);
       const int key0 = tile * kBN + warp * 16;   // this warp's first key
 
-      float z[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      // Two accumulators per 8 keys: a chain of D / 16 dependent MMAs is half as long.
+      float z[2][4], y[2][4];
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
         const uint32_t row = warp * 16 + nt * 8 + g;
@@ -292,34 +371,31 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         for (int i = 0; i < D / 64; ++i)
           x[i] = *reinterpret_cast<const uint4*>(kt + code_offset<D>(row, t4 * (D / 64) + i));
 #pragma unroll
+        for (int e = 0; e < 4; ++e) z[nt][e] = y[nt][e] = 0.f;
+#pragma unroll
         for (int i = 0; i < D / 64; ++i) {
           const uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             uint32_t lo, hi;
             codes_to_16bit<__half>(word[w], lo, hi);
-            mma_16816<__half>(z[nt], qa[4 * i + w], lo, hi);
+            mma_16816<__half>((w & 1) ? y[nt] : z[nt], qa[4 * i + w], lo, hi);
           }
         }
       }
-      // Keys nt * 8 + 2 t4 + {0, 1} of this warp: mult, log2 sv, 1 / sv.
+      // Keys nt * 8 + 2 t4 + {0, 1} of this warp.
       float2 inv[2];
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
-        const int at = warp * 16 + nt * 8 + 2 * t4;
-        const float2 sk = *reinterpret_cast<const float2*>(scales + at);
-        float2 sv = *reinterpret_cast<const float2*>(scales + kBN + at);
-        sv.x = sv.x < kMinScale ? kMinScale : sv.x;
-        sv.y = sv.y < kMinScale ? kMinScale : sv.y;
-        const float add0 = __log2f(sv.x), add1 = __log2f(sv.y);
-        // A scale that is not finite reaches the rows that see its key through z only.
-        inv[nt].x = sv.x <= 0x1p+127f ? __frcp_rn(sv.x) : 0.f;
-        inv[nt].y = sv.y <= 0x1p+127f ? __frcp_rn(sv.y) : 0.f;
+        const float* at = scales + warp * 16 + nt * 8 + 2 * t4;
+        const float2 sk = *reinterpret_cast<const float2*>(at);
+        const float2 add = *reinterpret_cast<const float2*>(at + kBN);
+        inv[nt] = *reinterpret_cast<const float2*>(at + 2 * kBN);
         const int key = key0 + nt * 8 + 2 * t4;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float z0 = fmaf(z[nt][2 * r] * row_scale[r], sk.x, add0);
-          const float z1 = fmaf(z[nt][2 * r + 1] * row_scale[r], sk.y, add1);
+          const float z0 = fmaf((z[nt][2 * r] + y[nt][2 * r]) * row_scale[r], sk.x, add.x);
+          const float z1 = fmaf((z[nt][2 * r + 1] + y[nt][2 * r + 1]) * row_scale[r], sk.y, add.y);
           z[nt][2 * r] = key < limit[r] ? z0 : -INFINITY;
           z[nt][2 * r + 1] = key + 1 < limit[r] ? z1 : -INFINITY;
         }
@@ -481,6 +557,13 @@ int launch_extend_few(const ExtendArgs& args, const flb_kv_cache* c, const void*
                       int64_t q_row_stride, int64_t q_head_stride, int dtype, int ctas, int dev,
                       cudaStream_t stream) {
   ExtendArgs a = args;
+  // Four keys' scales as one 16-byte load: contiguous along the keys and aligned at every fourth
+  // key (a page, like a tile, starts at a multiple of 4 keys).
+  auto wide = [](const float* base, const int64_t (&stride)[3]) {
+    return reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride[1] == 1 && stride[0] % 4 == 0 &&
+           stride[2] % 4 == 0;
+  };
+  a.wide_scales = wide(a.cache.ks, a.cache.ks_stride) && wide(a.cache.vs, a.cache.vs_stride);
   const QueryView qv{q, {q_row_stride, q_head_stride}};
   CUtensorMap tmk, tmv;
   const int d = c->head_dim;

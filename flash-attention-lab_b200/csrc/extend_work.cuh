@@ -33,6 +33,7 @@ struct ExtendArgs {
   int heads, group, causal;
   int tile_tokens;                    // tokens per tile: (128, or 16 in extend_few.cu) / group
   int select;                         // kAllRows, or which sequences this launch takes
+  int wide_scales;                    // extend_few.cu: scales are read 16 bytes at a time
   int box_rows;                       // cache rows per TMA box (a box never crosses a page)
   float scale_log2;
   TmaCoords kc, vc;

@@ -360,7 +360,9 @@ KvView kv_view(const flb_kv_cache* c) {
   }
   v.block_tables = c->block_tables;
   v.bt_stride = c->block_table_stride;
-  v.page_size = c->page_size;
+  const bool paged = c->block_tables != nullptr;
+  v.page = FastDiv::of(paged ? c->page_size : 1);
+  v.max_blocks = paged ? c->max_seqlen / c->page_size : 0;
   v.num_blocks = c->num_blocks;
   v.max_seqlen = c->max_seqlen;
   v.heads_kv = c->heads_kv;

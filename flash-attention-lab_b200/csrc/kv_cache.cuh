@@ -8,6 +8,24 @@
 
 namespace flb {
 
+// Division of 0 <= n < 2^31 by a constant d >= 1: with 2^(shift - 1) < d <= 2^shift and
+// mul = floor(2^32 (2^shift - d) / d) + 1, n / d = (n + (n mul >> 32)) >> shift.
+struct FastDiv {
+  uint32_t mul;
+  int shift, d;
+
+  static FastDiv of(int d) {
+    FastDiv f{0, 0, d};
+    while ((int64_t{1} << f.shift) < d) ++f.shift;
+    f.mul = static_cast<uint32_t>(((uint64_t{1} << 32) * ((uint64_t{1} << f.shift) - d)) / d + 1);
+    return f;
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return static_cast<int>((static_cast<uint32_t>(n) + __umulhi(static_cast<uint32_t>(n), mul)) >>
+                            shift);
+  }
+};
+
 // A KV cache as the kernels see it. Strides in elements of the cache (or of the scales).
 struct KvView {
   void* k;
@@ -18,7 +36,8 @@ struct KvView {
   int64_t ks_stride[3], vs_stride[3];
   const int32_t* block_tables;        // null: contiguous
   int64_t bt_stride;
-  int page_size, num_blocks, max_seqlen, heads_kv, batch;
+  FastDiv page;                       // page_size (1 when contiguous)
+  int num_blocks, max_blocks, max_seqlen, heads_kv, batch;
 
   // The (outer, row) of key `pos` of sequence b; false when it lies outside the cache.
   __device__ __forceinline__ bool locate(int b, int pos, int64_t& outer, int64_t& row) const {
@@ -26,11 +45,11 @@ struct KvView {
     outer = b;
     row = pos;
     if (block_tables != nullptr) {
-      const int page = pos / page_size;
-      const int blk = __ldg(block_tables + b * bt_stride + page);
+      const int p = page.div(pos);
+      const int blk = __ldg(block_tables + b * bt_stride + p);
       if (blk < 0 || blk >= num_blocks) return false;
       outer = blk;
-      row = pos - page * page_size;
+      row = pos - p * page.d;
     }
     return true;
   }
