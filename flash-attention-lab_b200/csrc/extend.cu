@@ -82,7 +82,7 @@ struct Geometry {
   static constexpr int kOtherRegs = kInt8 ? 56 : 72;
   static_assert(2 * 128 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs <= kThreads * kLaunchRegs,
                 "the register split must fit in the launch's registers");
-  static_assert((kMaxBatch + 1) * 8 <= kSlots * kTileBytes, "prefix sums fit in the ring");
+  static_assert(kMaxBatch * 8 <= kSlots * kTileBytes, "prefix sums fit in the rings");
 };
 
 template <int kKSlots, int kVSlots, int kCodeSlots>
@@ -1101,7 +1101,7 @@ extern "C" int flb_extend_fwd(const flb_kv_cache* c, const flb_extend_params* p,
   const bool many = !few || !known;
   if (few) {
     ExtendArgs f = a;
-    f.tile_tokens = kFewTile / a.group;
+    f.tile_tokens = many ? kFewTile / a.group : static_cast<int>(per_seq);
     f.select = many ? kFewRows : kAllRows;
     set_partials(&f, ws, sm_count, kFewTile);
     if (int st = launch_extend_few(f, c, p->q, p->q_row_stride, p->q_head_stride, p->dtype,

@@ -5,17 +5,23 @@
 // tcgen05 form of extend.cu took 297 us for 8 sequences of 24K keys, H_kv 8, D 128).
 //
 //  * One CTA per SM: one warp streams [128 keys x D] tiles of K and V codes by TMA, another turns the
-//    keys' scales into what the scores need (below) beside them in the ring stage, and eight
-//    consumer warps take 16 keys of every tile, each with its own online softmax; their results
-//    are joined in a fixed order at the end of a segment. Block tables are read 32 entries at a
-//    time. (One producer warp for copies and scales, with a table load per key, bounded 16-row
+//    keys' scales into what the scores need (below) beside them in the ring stage, and consumer
+//    warps take 16 keys of a tile each (two groups of eight warps on alternate tiles, or one),
+//    every warp with its own online softmax; their results are joined in a fixed order at the
+//    end of a segment. Block tables are read 32 entries at a time. (One producer warp for copies and scales, with a table load per key, bounded 16-row
 //    pages: 5000 clocks per tile where the consumers took 2400.)
-//  * Q is the A operand (rows = tokens x heads), in fp16: bf16 queries are scaled to [1, 2) of
-//    their row's maximum by a power of two, which is exact down to 2^-17 of the maximum and off by at
-//    most 2^-25 of it below. The order of a dot product is free, so thread t of a quad takes D / 4
-//    consecutive values of its key's row (16-byte shared loads) and the same ones of Q.
-//  * V goes through transposed 8 x 8 matrix loads of byte pairs: a register then holds columns d and
-//    d + 1 of two keys, one fragment for the even and one for the odd columns.
+//  * Keys are the M rows of the MMAs and score rows their N columns, in one or two blocks of 8: the
+//    usual group of up to 8 heads costs half the MMAs, exponentials and registers of 16 score rows,
+//    and the registers buy the second group of consumers, without which latency bound the
+//    kernel (2.5 warps per scheduler, 40 % of the issue slots, 1900 clocks per tile against the
+//    1400 that HBM needs).
+//  * Q is the B operand, in fp16: bf16 queries are scaled to [1, 2) of their row's maximum by a
+//    power of two, which is exact down to 2^-17 of the maximum and off by at most 2^-25 of it
+//    below. The order of a dot product is free, so thread t of a quad takes D / 4 consecutive values
+//    of its keys' rows (16-byte shared loads) and the same ones of Q.
+//  * V^T is the A operand of O^T = V^T P^T, by transposed 8 x 8 matrix loads of byte pairs: a
+//    register then holds columns d and d + 1 of two keys, M rows g and g + 8 of the fragment. P
+//    becomes the B operand by an 8 x 8 transpose in registers.
 //  * The scales act as in extend.cu: z = s mult + log2 sv, w = 2^(z - M) in fp16, the row sum takes
 //    w / sv.
 #include <algorithm>
@@ -25,22 +31,28 @@
 namespace flb {
 namespace {
 
-constexpr int kWarps = 8;             // consumers: 16 keys of a tile each
-constexpr int kCopyWarp = kWarps;      // TMA of the codes
-constexpr int kScaleWarp = kWarps + 1;
-constexpr int kFewThreads = (kWarps + 2) * 32;
-static_assert(kWarps * 16 == kBN, "the consumers cover a tile");
+constexpr int kGroupWarps = 8;        // consumers of one tile: 16 keys each
+static_assert(kGroupWarps * 16 == kBN, "a group covers a tile");
 
-template <int D>
+// kBlocks: 8-row blocks of score rows (1 or 2).
+template <int D, int kBlocks>
 struct FewGeometry {
-  static constexpr int kTileBytes = kBN * D;          // K or V codes
-  static constexpr int kStages = D == 128 ? 4 : 8;    // 128 KB of codes
+  static constexpr int kRows = 8 * kBlocks;
+  static constexpr int kGroups = 1;   // consumer groups, on alternate tiles
+  static constexpr int kWarps = kGroups * kGroupWarps;
+  static constexpr int kCopyWarp = kWarps;               // TMA of the codes
+  static constexpr int kScaleWarp = kWarps + 1;
+  static constexpr int kThreads = (kWarps + 2) * 32;
+  static constexpr int kTileBytes = kBN * D;             // K or V codes
+  static constexpr int kStages = D == 128 ? 4 : 8;       // 128 KB of codes
   static constexpr int kScaleOffset = kStages * 2 * kTileBytes;
-  static constexpr int kScaleBytes = 3 * kBN * 4;     // sk, log2 sv and 1 / sv of one stage
-  static constexpr int kJoinOffset = kScaleOffset + kStages * kScaleBytes;
-  static constexpr int kJoinBytes = kWarps * kFewTile * (D + 2) * 4;
+  static constexpr int kScaleBytes = 3 * kBN * 4;        // sk, log2 sv and 1 / sv of one stage
+  static constexpr int kRawTiles = 8;                    // scales as read: see the scale warp
+  static constexpr int kRawOffset = kScaleOffset + kStages * kScaleBytes;
+  static constexpr int kJoinOffset = kRawOffset + kRawTiles * 2 * kBN * 4;
+  static constexpr int kJoinBytes = kWarps * kRows * (D + 2) * 4;
   static constexpr int kTailOffset = kJoinOffset + kJoinBytes;
-  static_assert((kMaxBatch + 1) * 8 <= kScaleOffset, "prefix sums fit in the ring");
+  static_assert(kMaxBatch * 8 <= kScaleOffset, "prefix sums fit in the ring");
 };
 
 template <int kStages>
@@ -50,6 +62,16 @@ struct FewShared {
   int abort_flag;
   Share share;
 };
+
+// Copies 16 or 4 bytes to shared memory (the shorter form: zeros unless valid).
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const float* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const float* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
+               "r"(valid ? 4 : 0)
+               : "memory");
+}
 
 __device__ __forceinline__ float lg2(float x) {
   float y;
@@ -111,7 +133,16 @@ __device__ __forceinline__ void code_columns(uint32_t x, uint32_t& even, uint32_
   odd = *reinterpret_cast<uint32_t*>(&r);
 }
 
-// True on all consumer threads when pred holds on any of them.
+// The 8 x 8 matrix of 16-bit values that a warp holds (row lane / 4, columns 2 (lane % 4) + {0, 1}),
+// transposed.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// True on all kThreads consumer threads when pred holds on any of them.
+template <int kThreads>
 __device__ __forceinline__ bool consumers_any(bool pred) {
   uint32_t r;
   asm volatile(
@@ -120,7 +151,7 @@ __device__ __forceinline__ bool consumers_any(bool pred) {
       "bar.red.or.pred q, 1, %2, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(static_cast<uint32_t>(pred)), "n"(kWarps * 32)
+      : "r"(static_cast<uint32_t>(pred)), "n"(kThreads)
       : "memory");
   return r != 0;
 }
@@ -130,16 +161,17 @@ struct QueryView {
   int64_t stride[2];   // row, head
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kFewThreads, 1)
+template <typename T, int D, int kBlocks>
+__global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
     extend_few_kernel(const __grid_constant__ ExtendArgs a, const __grid_constant__ QueryView qv,
                       const __grid_constant__ CUtensorMap tmk,
                       const __grid_constant__ CUtensorMap tmv) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  using G = FewGeometry<D>;
+  using G = FewGeometry<D, kBlocks>;
   constexpr int kStages = G::kStages;
-  constexpr int kSteps = D / 16;    // MMA steps over head_dim
-  constexpr int kCols = D / 8;      // 8-column blocks of O
+  constexpr int kWarps = G::kWarps;
+  constexpr int kRows = G::kRows;
+  constexpr int kSteps = D / 16;    // MMA steps over head_dim, and 16-column chunks of V
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -151,11 +183,11 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     sh->abort_flag = 0;
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sh->full[i], 33);   // the TMA bytes and each lane's scales
-      mbar_init(&sh->empty[i], kWarps);
+      mbar_init(&sh->empty[i], kGroupWarps);
     }
     fence_barrier_init();
   }
-  if (warp == kCopyWarp && lane == 0) {
+  if (warp == G::kCopyWarp && lane == 0) {
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
   }
@@ -167,7 +199,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   Segment s;
   walk.start(a, sh->share);
 
-  if (warp == kCopyWarp) {
+  if (warp == G::kCopyWarp) {
     // ------------------------------- copies -------------------------------
     // Lane i issues copy i of a tile: a part of box_rows rows, of K or of V.
     const int parts = kBN / a.box_rows;
@@ -210,50 +242,69 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     }
     return;
   }
-  if (warp == kScaleWarp) {
+  if (warp == G::kScaleWarp) {
     // ------------------------------- scales -------------------------------
-    // Lane i turns the scales of keys 4 i .. 4 i + 3 of a tile, read one tile ahead, into sk,
-    // log2 sv and 1 / sv. They lie in one page. With a.wide_scales they are 16 contiguous bytes.
+    // Lane i turns the scales of keys 4 i .. 4 i + 3 of a tile into sk, log2 sv and 1 / sv. They lie
+    // in one page, as 16 contiguous bytes with a.wide_scales. They are copied to shared memory
+    // kRawTiles - 1 tiles ahead, each lane its own: a warp alone runs about 5 clocks per instruction
+    // and cannot wait for memory in every tile (registers one tile ahead: 2200 clocks per
+    // tile, where the consumers take 950).
+    constexpr int kRawTiles = G::kRawTiles;
     const bool paged = a.cache.block_tables != nullptr;
     const int64_t ks_row = a.cache.ks_stride[1], vs_row = a.cache.vs_stride[1];
+    const uint32_t raw = smem_u32(smem + G::kRawOffset) + lane * 16;
     BlockWindow window;
     int issued = 0;
     bool ok = true;
     while (ok && walk.next(a, s)) {
       if (paged) window.start(a.cache, s.b, a.cache.page.div(s.t0 * kBN), lane);
+      const float* ks = a.cache.ks + s.hkv * a.cache.ks_stride[2];
+      const float* vs = a.cache.vs + s.hkv * a.cache.vs_stride[2];
+      if (!paged) {
+        ks += s.b * a.cache.ks_stride[0];
+        vs += s.b * a.cache.vs_stride[0];
+      }
       // Keys past the length are not read: they stay hidden, whatever their scales.
-      auto fetch = [&](int tile, float (&sk)[4], float (&sv)[4]) {
-        const int key = tile * kBN + 4 * lane;
-        int64_t outer = s.b, row = key;
-        if (paged) {
-          const int page = a.cache.page.div(key);
-          window.advance(a.cache, __shfl_sync(0xffffffffu, page, 0), lane);
-          outer = window.at(page);
-          row = key - page * a.cache.page.d;
-        }
-        const int keys = outer >= 0 ? s.seq.len - key : 0;
-        const float* k = a.cache.ks + outer * a.cache.ks_stride[0] + row * ks_row +
-                         s.hkv * a.cache.ks_stride[2];
-        const float* v = a.cache.vs + outer * a.cache.vs_stride[0] + row * vs_row +
-                         s.hkv * a.cache.vs_stride[2];
-        if (a.wide_scales && keys >= 4) {
-          const float4 x = __ldg(reinterpret_cast<const float4*>(k));
-          const float4 y = __ldg(reinterpret_cast<const float4*>(v));
-          sk[0] = x.x, sk[1] = x.y, sk[2] = x.z, sk[3] = x.w;
-          sv[0] = y.x, sv[1] = y.y, sv[2] = y.z, sv[3] = y.w;
-        } else {
+      auto fetch = [&](int tile) {
+        if (tile < s.t1) {
+          const int key = tile * kBN + 4 * lane;
+          const float *k = ks, *v = vs;
+          int row = key, keys = s.seq.len - key;
+          if (paged) {
+            const int page = a.cache.page.div(key);
+            window.advance(a.cache, __shfl_sync(0xffffffffu, page, 0), lane);
+            const int blk = window.at(page);
+            if (blk < 0) keys = 0;
+            k += max(blk, 0) * a.cache.ks_stride[0];
+            v += max(blk, 0) * a.cache.vs_stride[0];
+            row = key - page * a.cache.page.d;
+          }
+          k += row * ks_row;
+          v += row * vs_row;
+          const uint32_t dst = raw + (tile - s.t0) % kRawTiles * (2 * kBN * 4);
+          if (a.wide_scales && keys >= 4) {
+            cp_async_16(dst, k);
+            cp_async_16(dst + kBN * 4, v);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sk[i] = i < keys ? __ldg(k + i * ks_row) : 0.f;
-            sv[i] = i < keys ? __ldg(v + i * vs_row) : kMinScale;
+            for (int i = 0; i < 4; ++i) {
+              const bool in = i < keys;
+              cp_async_4(dst + 4 * i, in ? k + i * ks_row : a.cache.ks, in);
+              cp_async_4(dst + kBN * 4 + 4 * i, in ? v + i * vs_row : a.cache.vs, in);
+            }
           }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      float sk[4], sv[4];
-      if (s.t0 < s.t1) fetch(s.t0, sk, sv);
+      for (int i = 0; i < kRawTiles - 1; ++i) fetch(s.t0 + i);
       for (int tile = s.t0; tile < s.t1; ++tile) {
-        float sk_next[4] = {0.f, 0.f, 0.f, 0.f}, sv_next[4] = {0.f, 0.f, 0.f, 0.f};
-        if (tile + 1 < s.t1) fetch(tile + 1, sk_next, sv_next);
+        fetch(tile + kRawTiles - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRawTiles - 1) : "memory");
+        const float4* from = reinterpret_cast<const float4*>(
+            smem + G::kRawOffset + (tile - s.t0) % kRawTiles * (2 * kBN * 4)) + lane;
+        const float4 sk = from[0];
+        const float4 sv4 = from[kBN / 4];
+        const float sv[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
         const int st = issued % kStages;
         ok = issued < kStages || mbar_wait(&sh->empty[st], ((issued / kStages) - 1) & 1, guard);
         ok = __all_sync(0xffffffffu, ok);
@@ -267,17 +318,13 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           inv[i] = v <= 0x1p+127f ? rcp(v) : 0.f;
         }
         float4* dst = reinterpret_cast<float4*>(smem + G::kScaleOffset + st * G::kScaleBytes) + lane;
-        dst[0] = make_float4(sk[0], sk[1], sk[2], sk[3]);
+        dst[0] = sk;
         dst[kBN / 4] = make_float4(add[0], add[1], add[2], add[3]);
         dst[2 * (kBN / 4)] = make_float4(inv[0], inv[1], inv[2], inv[3]);
         mbar_arrive(&sh->full[st]);
         ++issued;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sk[i] = sk_next[i];
-          sv[i] = sv_next[i];
-        }
       }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     zero_other_rows<T, D>(a, blockIdx.x, gridDim.x, lane);
     return;
@@ -286,39 +333,41 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   // ------------------------------- consumers -------------------------------
   const int g = lane >> 2;    // fragment row group
   const int t4 = lane & 3;    // thread in quad
-  float* join_m = reinterpret_cast<float*>(smem + G::kJoinOffset);   // [warps][16]
-  float* join_l = join_m + kWarps * kFewTile;
-  float* join_o = join_l + kWarps * kFewTile;                        // [warps][16][D]
+  const int group = warp / kGroupWarps, slice = warp % kGroupWarps;   // tiles, and keys in a tile
+  float* join_m = reinterpret_cast<float*>(smem + G::kJoinOffset);   // [warps][kRows]
+  float* join_l = join_m + kWarps * kRows;
+  float* join_o = join_l + kWarps * kRows;                           // [warps][kRows][D]
   const uint32_t smem_base = smem_u32(smem);
-  const uint32_t v_row = static_cast<uint32_t>(warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7));
+  const uint32_t v_row = static_cast<uint32_t>(slice * 16 + ((lane >> 3) & 1) * 8 + (lane & 7));
   const uint32_t v_chunk = static_cast<uint32_t>(lane >> 4);
-  int done = 0;               // tiles consumed
+  int base = 0;               // tiles of earlier segments
   int segments = 0;
   int4 meta0 = make_int4(0, 0, 0, 0), meta1 = make_int4(0, 0, 0, 0);
   bool ok = true;
   while (walk.next(a, s)) {
     const bool first_segment = segments++ == 0;
     const int rows = s.tokens * a.group;
-    // Q fragments: rows g and g + 8, values [t4 D / 4, (t4 + 1) D / 4).
-    uint32_t qa[kSteps][4];
-    float row_scale[2] = {a.scale_log2, a.scale_log2};
-    int limit[2];             // keys that the row sees
+    // Q fragments: rows 8 nb + g, values [t4 D / 4, (t4 + 1) D / 4). Scores: this thread has rows
+    // 8 nb + 2 t4 + {0, 1} of keys g and g + 8.
+    uint32_t qb[kBlocks][kSteps][2];
+    float row_scale[kBlocks][2];
+    int limit[kBlocks][2];    // keys that the row sees
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = g + 8 * r;
+    for (int nb = 0; nb < kBlocks; ++nb) {
+      const int row = 8 * nb + g;
       const int token = row / a.group, head = s.hkv * a.group + row - token * a.group;
-      limit[r] = a.causal ? min(s.seq.len, s.seq.len - s.seq.n + s.first + token + 1) : s.seq.len;
       const uint2* src = reinterpret_cast<const uint2*>(
           static_cast<const T*>(qv.q) + (s.seq.row0 + s.first + token) * qv.stride[0] +
           head * qv.stride[1] + t4 * (D / 4));
       uint2 x[kSteps];
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) x[k] = row < rows ? __ldg(src + k) : make_uint2(0, 0);
+      float up = a.scale_log2;
       if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-          qa[k][r] = x[k].x;
-          qa[k][2 + r] = x[k].y;
+          qb[nb][k][0] = x[k].x;
+          qb[nb][k][1] = x[k].y;
         }
       } else {
         // The exponent of the row's maximum (magnitudes compare as integers).
@@ -332,152 +381,176 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int e = min(max(static_cast<int>(top >> 7), 1), 253);
         const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-        row_scale[r] *= __uint_as_float(static_cast<uint32_t>(e) << 23);
+        up *= __uint_as_float(static_cast<uint32_t>(e) << 23);
         auto half_pair = [&](uint32_t v) {
           return pack2<__half>(__uint_as_float(v << 16) * down,
                                __uint_as_float(v & 0xffff0000u) * down);
         };
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-          qa[k][r] = half_pair(x[k].x);
-          qa[k][2 + r] = half_pair(x[k].y);
+          qb[nb][k][0] = half_pair(x[k].x);
+          qb[nb][k][1] = half_pair(x[k].y);
         }
       }
-    }
-    float o[kCols][4];        // block 2 c + p: columns 16 c + 2 n + p of chunk c, n = 0..7
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m_ref[2] = {-INFINITY, -INFINITY};   // log2-domain reference points
-    float l_sum[2] = {0.f, 0.f};               // this thread's share of the row sums
+      for (int e = 0; e < 2; ++e) {
+        row_scale[nb][e] = __shfl_sync(0xffffffffu, up, (2 * t4 + e) * 4);
+        limit[nb][e] = a.causal ? min(s.seq.len, s.seq.len - s.seq.n + s.first +
+                                                     (8 * nb + 2 * t4 + e) / a.group + 1)
+                                : s.seq.len;
+      }
+    }
+    // O^T: columns 16 c + 2 g (elements 0, 1) and 16 c + 2 g + 1 (2, 3) of rows 8 nb + 2 t4 + {0, 1}.
+    float o[kBlocks][kSteps][4];
+    float m_ref[kBlocks][2], l_sum[kBlocks][2];   // log2-domain reference point; share of the sum
+#pragma unroll
+    for (int nb = 0; nb < kBlocks; ++nb) {
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c)
+        o[nb][c][0] = o[nb][c][1] = o[nb][c][2] = o[nb][c][3] = 0.f;
+      m_ref[nb][0] = m_ref[nb][1] = -INFINITY;
+      l_sum[nb][0] = l_sum[nb][1] = 0.f;
+    }
 
-    for (int tile = s.t0; ok && tile < s.t1; ++tile) {
-      const int st = done % kStages;
-      ok = mbar_wait(&sh->full[st], (done / kStages) & 1, guard);
+    // This group's tiles of the segment: those at ring positions of its parity.
+    const int skip = (group + G::kGroups - base % G::kGroups) % G::kGroups;
+    for (int tile = s.t0 + skip; tile < s.t1; tile += G::kGroups) {
+      const int pos = base + tile - s.t0, st = pos % kStages;
+      ok = mbar_wait(&sh->full[st], (pos / kStages) & 1, guard);
       if (!ok) break;
-      ++done;
       const uint8_t* kt = smem + 2 * st * G::kTileBytes;
       const uint32_t vt = smem_base + (2 * st + 1) * G::kTileBytes;
       const float* scales = reinterpret_cast<const float*>(smem + G::kScaleOffset +
-                                                           st * G::kScaleBytes);
-      const int key0 = tile * kBN + warp * 16;   // this warp's first key
+                                                           st * G::kScaleBytes) + slice * 16 + g;
+      const int key = tile * kBN + slice * 16 + g;   // and key + 8
 
-      // Two accumulators per 8 keys: a chain of D / 16 dependent MMAs is half as long.
-      float z[2][4], y[2][4];
+      // Two accumulators per block: a chain of D / 16 dependent MMAs is half as long.
+      float z[kBlocks][4], y[kBlocks][4];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const uint32_t row = warp * 16 + nt * 8 + g;
-        uint4 x[D / 64];
+      for (int nb = 0; nb < kBlocks; ++nb) {
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i)
-          x[i] = *reinterpret_cast<const uint4*>(kt + code_offset<D>(row, t4 * (D / 64) + i));
+        for (int e = 0; e < 4; ++e) z[nb][e] = y[nb][e] = 0.f;
+      }
+      {
+        uint4 x[2][D / 64];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[nt][e] = y[nt][e] = 0.f;
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i)
+            x[r][i] = *reinterpret_cast<const uint4*>(
+                kt + code_offset<D>(slice * 16 + 8 * r + g, t4 * (D / 64) + i));
+        }
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
-          const uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          const uint32_t word0[4] = {x[0][i].x, x[0][i].y, x[0][i].z, x[0][i].w};
+          const uint32_t word1[4] = {x[1][i].x, x[1][i].y, x[1][i].z, x[1][i].w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            uint32_t lo, hi;
-            codes_to_16bit<__half>(word[w], lo, hi);
-            mma_16816<__half>((w & 1) ? y[nt] : z[nt], qa[4 * i + w], lo, hi);
+            uint32_t ka[4];
+            codes_to_16bit<__half>(word0[w], ka[0], ka[2]);
+            codes_to_16bit<__half>(word1[w], ka[1], ka[3]);
+#pragma unroll
+            for (int nb = 0; nb < kBlocks; ++nb)
+              mma_16816<__half>((w & 1) ? y[nb] : z[nb], ka, qb[nb][4 * i + w][0],
+                                qb[nb][4 * i + w][1]);
           }
         }
       }
-      // Keys nt * 8 + 2 t4 + {0, 1} of this warp.
-      float2 inv[2];
+      const float sk[2] = {scales[0], scales[8]};
+      const float add[2] = {scales[kBN], scales[kBN + 8]};
+      const float inv[2] = {scales[2 * kBN], scales[2 * kBN + 8]};
+      // Element e: row e & 1, key g + 8 (e >> 1). The reference point moves only when a score
+      // passes it by more than 2^8, and the warp's maximum is taken only then.
+      bool above = false;
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const float* at = scales + warp * 16 + nt * 8 + 2 * t4;
-        const float2 sk = *reinterpret_cast<const float2*>(at);
-        const float2 add = *reinterpret_cast<const float2*>(at + kBN);
-        inv[nt] = *reinterpret_cast<const float2*>(at + 2 * kBN);
-        const int key = key0 + nt * 8 + 2 * t4;
+      for (int nb = 0; nb < kBlocks; ++nb) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float z0 = fmaf((z[nt][2 * r] + y[nt][2 * r]) * row_scale[r], sk.x, add.x);
-          const float z1 = fmaf((z[nt][2 * r + 1] + y[nt][2 * r + 1]) * row_scale[r], sk.y, add.y);
-          z[nt][2 * r] = key < limit[r] ? z0 : -INFINITY;
-          z[nt][2 * r + 1] = key + 1 < limit[r] ? z1 : -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+          const int r = e & 1, k = e >> 1;
+          const float v = fmaf((z[nb][e] + y[nb][e]) * row_scale[nb][r], sk[k], add[k]);
+          z[nb][e] = key + 8 * k < limit[nb][r] ? v : -INFINITY;
+          above |= z[nb][e] > m_ref[nb][r] + kRescaleThreshold;
         }
       }
-      float factor[2], ref[2];
-      bool rescale = false;
+      if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float mx = fmaxf(fmaxf(z[0][2 * r], z[0][2 * r + 1]), fmaxf(z[1][2 * r], z[1][2 * r + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // The reference point moves only when the maximum passes it by more than 2^8.
-        float m_new = m_ref[r];
-        if (m_new == -INFINITY || mx > m_new + kRescaleThreshold) m_new = fmaxf(m_new, mx);
-        factor[r] = 1.f;
-        if (m_new != m_ref[r]) {
-          factor[r] = ex2(m_ref[r] - m_new);   // 0 for the first keys
-          rescale = true;
-        }
-        m_ref[r] = m_new;
-        ref[r] = m_new == -INFINITY ? 0.f : m_new;
-      }
-      if (__any_sync(0xffffffffu, rescale)) {
-        l_sum[0] *= factor[0];
-        l_sum[1] *= factor[1];
+        for (int nb = 0; nb < kBlocks; ++nb) {
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) {
-          o[i][0] *= factor[0];
-          o[i][1] *= factor[0];
-          o[i][2] *= factor[1];
-          o[i][3] *= factor[1];
+          for (int r = 0; r < 2; ++r) {
+            float mx = fmaxf(z[nb][r], z[nb][2 + r]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            if (mx > m_ref[nb][r] + kRescaleThreshold) {
+              const float factor = ex2(m_ref[nb][r] - mx);   // 0 for the first keys
+              m_ref[nb][r] = mx;
+              l_sum[nb][r] *= factor;
+#pragma unroll
+              for (int c = 0; c < kSteps; ++c) {
+                o[nb][c][r] *= factor;
+                o[nb][c][2 + r] *= factor;
+              }
+            }
+          }
         }
       }
+      uint32_t pb[kBlocks][2];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
+      for (int nb = 0; nb < kBlocks; ++nb) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[nt][e] = ex2(z[nt][e] - ref[e >> 1]);
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          l_sum[r] = fmaf(z[nt][2 * r], inv[nt].x, fmaf(z[nt][2 * r + 1], inv[nt].y, l_sum[r]));
+        for (int e = 0; e < 4; ++e) {
+          const int r = e & 1;
+          const float ref = m_ref[nb][r] == -INFINITY ? 0.f : m_ref[nb][r];
+          z[nb][e] = ex2(z[nb][e] - ref);
+          l_sum[nb][r] = fmaf(z[nb][e], inv[e >> 1], l_sum[nb][r]);
+        }
+        pb[nb][0] = transpose8x8(pack2<__half>(z[nb][0], z[nb][1]));
+        pb[nb][1] = transpose8x8(pack2<__half>(z[nb][2], z[nb][3]));
       }
-      const uint32_t pa[4] = {pack2<__half>(z[0][0], z[0][1]), pack2<__half>(z[0][2], z[0][3]),
-                              pack2<__half>(z[1][0], z[1][1]), pack2<__half>(z[1][2], z[1][3])};
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t v[4];   // keys 0-7 and 8-15 of chunk 2 c, then of chunk 2 c + 1
-        ldsm_x4_trans(vt + code_offset<D>(v_row, 2 * c + v_chunk), v[0], v[1], v[2], v[3]);
+      for (int c = 0; c < kSteps; c += 2) {
+        uint32_t v[4];   // keys 0-7 and 8-15 of chunk c, then of chunk c + 1
+        ldsm_x4_trans(vt + code_offset<D>(v_row, c + v_chunk), v[0], v[1], v[2], v[3]);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t even0, odd0, even1, odd1;
-          code_columns(v[2 * half], even0, odd0);
-          code_columns(v[2 * half + 1], even1, odd1);
-          mma_16816<__half>(o[2 * (2 * c + half)], pa, even0, even1);
-          mma_16816<__half>(o[2 * (2 * c + half) + 1], pa, odd0, odd1);
+        for (int i = 0; i < 2; ++i) {
+          uint32_t va[4];
+          code_columns(v[2 * i], va[0], va[1]);
+          code_columns(v[2 * i + 1], va[2], va[3]);
+#pragma unroll
+          for (int nb = 0; nb < kBlocks; ++nb)
+            mma_16816<__half>(o[nb][c + i], va, pb[nb][0], pb[nb][1]);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->empty[st]);
     }
+    base += s.t1 - s.t0;
 
     // Join the warps. Every consumer is past the previous segment's reads after the first barrier.
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 1);
-      l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 2);
-    }
-    if (consumers_any(!ok || *guard.abort_flag != 0)) break;
+    for (int nb = 0; nb < kBlocks; ++nb) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = g + 8 * r;
-      if (row >= rows) continue;
-      if (t4 == 0) {
-        join_m[warp * kFewTile + row] = m_ref[r];
-        join_l[warp * kFewTile + row] = l_sum[r];
+      for (int r = 0; r < 2; ++r) {
+        l_sum[nb][r] += __shfl_xor_sync(0xffffffffu, l_sum[nb][r], 4);
+        l_sum[nb][r] += __shfl_xor_sync(0xffffffffu, l_sum[nb][r], 8);
+        l_sum[nb][r] += __shfl_xor_sync(0xffffffffu, l_sum[nb][r], 16);
       }
-      float* dst = join_o + (warp * kFewTile + row) * D;
+    }
+    if (consumers_any<kWarps * 32>(!ok || *guard.abort_flag != 0)) break;
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        // Columns 16 c + 4 t4 + {0, 1, 2, 3}: even and odd blocks interleaved.
-        *reinterpret_cast<float4*>(dst + 16 * c + 4 * t4) =
-            make_float4(o[2 * c][2 * r], o[2 * c + 1][2 * r], o[2 * c][2 * r + 1],
-                        o[2 * c + 1][2 * r + 1]);
+    for (int nb = 0; nb < kBlocks; ++nb) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = 8 * nb + 2 * t4 + r;
+        if (row >= rows) continue;
+        if (g == 0) {
+          join_m[warp * kRows + row] = m_ref[nb][r];
+          join_l[warp * kRows + row] = l_sum[nb][r];
+        }
+        float* dst = join_o + (warp * kRows + row) * D + 2 * g;
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c)
+          *reinterpret_cast<float2*>(dst + 16 * c) = make_float2(o[nb][c][r], o[nb][c][2 + r]);
       }
     }
     asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
@@ -487,14 +560,14 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       const int row = idx / (D / 4), col = (idx % (D / 4)) * 4;
       float m = -INFINITY, l = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, join_m[w * kFewTile + row]);
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, join_m[w * kRows + row]);
       const float top = m == -INFINITY ? 0.f : m;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2(join_m[w * kFewTile + row] - top);
-        const float4 x = *reinterpret_cast<const float4*>(join_o + (w * kFewTile + row) * D + col);
-        l = fmaf(join_l[w * kFewTile + row], f, l);
+        const float f = ex2(join_m[w * kRows + row] - top);
+        const float4 x = *reinterpret_cast<const float4*>(join_o + (w * kRows + row) * D + col);
+        l = fmaf(join_l[w * kRows + row], f, l);
         acc.x = fmaf(x.x, f, acc.x);
         acc.y = fmaf(x.y, f, acc.y);
         acc.z = fmaf(x.z, f, acc.z);
@@ -532,23 +605,34 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int kBlocks>
 int launch(const ExtendArgs& a, const QueryView& qv, const CUtensorMap& tmk, const CUtensorMap& tmv,
            int ctas, int dev, cudaStream_t stream) {
-  using G = FewGeometry<D>;
+  using G = FewGeometry<D, kBlocks>;
   constexpr int kSmem = G::kTailOffset + static_cast<int>(sizeof(FewShared<G::kStages>)) + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
   static thread_local int configured_device = -1;
   if (configured_device != dev) {
-    if (int st = check_cuda(cudaFuncSetAttribute(extend_few_kernel<T, D>,
+    if (int st = check_cuda(cudaFuncSetAttribute(extend_few_kernel<T, D, kBlocks>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  kSmem),
                             "cudaFuncSetAttribute(extend few)"))
       return st;
     configured_device = dev;
   }
-  extend_few_kernel<T, D><<<ctas, kFewThreads, kSmem, stream>>>(a, qv, tmk, tmv);
+  extend_few_kernel<T, D, kBlocks><<<ctas, G::kThreads, kSmem, stream>>>(a, qv, tmk, tmv);
   return check_cuda(cudaGetLastError(), "extend_few_kernel launch");
+}
+
+template <typename T>
+int launch_t(const ExtendArgs& a, const QueryView& qv, const CUtensorMap& tmk,
+             const CUtensorMap& tmv, int head_dim, int rows, int ctas, int dev,
+             cudaStream_t stream) {
+  if (head_dim == 128)
+    return rows <= 8 ? launch<T, 128, 1>(a, qv, tmk, tmv, ctas, dev, stream)
+                     : launch<T, 128, 2>(a, qv, tmk, tmv, ctas, dev, stream);
+  return rows <= 8 ? launch<T, 64, 1>(a, qv, tmk, tmv, ctas, dev, stream)
+                   : launch<T, 64, 2>(a, qv, tmk, tmv, ctas, dev, stream);
 }
 
 }  // namespace
@@ -571,11 +655,10 @@ int launch_extend_few(const ExtendArgs& args, const flb_kv_cache* c, const void*
     return st;
   if (int st = encode_rows_map(&tmv, &a.vc, kv_view4(c, true), a.box_rows, d, FLB_INT8, d))
     return st;
+  const int rows = a.tile_tokens * a.group;   // the most score rows of a sequence
   if (dtype == FLB_BF16)
-    return d == 128 ? launch<__nv_bfloat16, 128>(a, qv, tmk, tmv, ctas, dev, stream)
-                    : launch<__nv_bfloat16, 64>(a, qv, tmk, tmv, ctas, dev, stream);
-  return d == 128 ? launch<__half, 128>(a, qv, tmk, tmv, ctas, dev, stream)
-                  : launch<__half, 64>(a, qv, tmk, tmv, ctas, dev, stream);
+    return launch_t<__nv_bfloat16>(a, qv, tmk, tmv, d, rows, ctas, dev, stream);
+  return launch_t<__half>(a, qv, tmk, tmv, d, rows, ctas, dev, stream);
 }
 
 }  // namespace flb

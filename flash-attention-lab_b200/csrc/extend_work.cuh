@@ -183,11 +183,105 @@ struct Walk {
   }
 };
 
-// Finds this CTA's share. All threads; `pref` is shared memory for batch + 1 values.
+// x / y for 0 <= x, 0 < y: 32-bit where both fit (a 64-bit division takes hundreds of clocks).
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
+  return ((x | y) >> 31) != 0 ? x / y
+                              : static_cast<int64_t>(static_cast<uint32_t>(x) /
+                                                     static_cast<uint32_t>(y));
+}
+
+// Units of a sequence's items of one KV head, by a whole warp.
+__device__ __forceinline__ int64_t sequence_units(const ExtendArgs& a, const Sequence& s, int lane) {
+  const int n = items_of(a, s);
+  int64_t sum = 0;
+  for (int k = lane; k < n; k += 32) sum += item_units(a, s, k);
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+
+// The share's start: unit `rem` of sequence b, whose units over all heads are `own`. One warp.
+__device__ __forceinline__ void locate_unit(const ExtendArgs& a, Share* sh, int b, const Sequence& s,
+                                            int64_t own, int64_t rem, int lane) {
+  const int64_t per_head = divide(own, a.cache.heads_kv);
+  const int hkv = static_cast<int>(divide(rem, per_head));
+  rem -= hkv * per_head;
+  const int n = items_of(a, s);
+  int64_t before = 0;
+  int k = 0;
+  for (int k0 = 0; n > 1 && k0 < n; k0 += 32) {
+    const int64_t u = k0 + lane < n ? item_units(a, s, k0 + lane) : 0;
+    int64_t incl = u;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, before + incl > rem);
+    if (past != 0) {
+      const int at = __ffs(past) - 1;
+      before += __shfl_sync(0xffffffffu, incl - u, at);
+      k = k0 + at;
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (lane == 0) {
+    sh->b = b;
+    sh->hkv = hkv;
+    sh->k = k;
+    sh->at = static_cast<int>(rem - before);
+  }
+}
+
+// Units [g0, g1) of CTA c: shares differ by at most one unit.
+__device__ __forceinline__ void share_bounds(int64_t total, int64_t& g0, int64_t& g1) {
+  const int64_t ctas = gridDim.x, c = blockIdx.x;
+  const int64_t each = divide(total, ctas), more = total - each * ctas;
+  g0 = each * c + min(c, more);
+  g1 = g0 + each + (c < more ? 1 : 0);
+}
+
+// Finds this CTA's share. All threads; `pref` is shared memory for batch values. It ends without a
+// barrier. Up to 32 sequences are one warp's work (a lane per sequence), which the start of a
+// short call waits for; more go through shared memory.
 __device__ __forceinline__ void find_share(const ExtendArgs& a, Share* sh, int64_t* pref) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int batch = a.ragged.batch;
   constexpr int kFew = 4;   // items one thread sums by itself
+  int64_t g0, g1;
+  if (batch <= 32) {
+    if (warp != 0) return;
+    Sequence s{0, 0, 0};
+    if (lane < batch) s = load_sequence(a, lane);
+    const int n = items_of(a, s);
+    int64_t own = 0;
+    if (n <= kFew) {
+      for (int k = 0; k < n; ++k) own += item_units(a, s, k);
+    }
+    for (uint32_t long_ones = __ballot_sync(0xffffffffu, n > kFew); long_ones != 0;
+         long_ones &= long_ones - 1) {
+      const int b = __ffs(long_ones) - 1;
+      const Sequence t{__shfl_sync(0xffffffffu, s.row0, b), __shfl_sync(0xffffffffu, s.n, b),
+                       __shfl_sync(0xffffffffu, s.len, b)};
+      const int64_t sum = sequence_units(a, t, lane);
+      if (lane == b) own = sum;
+    }
+    own *= a.cache.heads_kv;
+    int64_t incl = own;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    share_bounds(__shfl_sync(0xffffffffu, incl, 31), g0, g1);
+    if (g1 > g0) {
+      const int b = __ffs(__ballot_sync(0xffffffffu, incl > g0)) - 1;
+      const Sequence t{__shfl_sync(0xffffffffu, s.row0, b), __shfl_sync(0xffffffffu, s.n, b),
+                       __shfl_sync(0xffffffffu, s.len, b)};
+      const int64_t units = __shfl_sync(0xffffffffu, own, b);
+      locate_unit(a, sh, b, t, units, g0 - (__shfl_sync(0xffffffffu, incl, b) - units), lane);
+    }
+    if (lane == 0) sh->units = g1 - g0;
+    return;
+  }
   for (int b = threadIdx.x; b < batch; b += blockDim.x) {
     const Sequence s = load_sequence(a, b);
     const int n = items_of(a, s);
@@ -198,75 +292,38 @@ __device__ __forceinline__ void find_share(const ExtendArgs& a, Share* sh, int64
   __syncthreads();
   for (int b = warp; b < batch; b += blockDim.x >> 5) {
     if (pref[b] != -1) continue;
-    const Sequence s = load_sequence(a, b);
-    const int n = items_of(a, s);
-    int64_t sum = 0;
-    for (int k = lane; k < n; k += 32) sum += item_units(a, s, k);
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const int64_t sum = sequence_units(a, load_sequence(a, b), lane);
     __syncwarp();
     if (lane == 0) pref[b] = sum * a.cache.heads_kv;
   }
   __syncthreads();
-  if (warp == 0) {
-    // Exclusive prefix sums in place; pref[batch] is the total.
-    int64_t run = 0;
-    for (int b0 = 0; b0 < batch; b0 += 32) {
-      const int64_t own = b0 + lane < batch ? pref[b0 + lane] : 0;
-      int64_t incl = own;
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      if (b0 + lane < batch) pref[b0 + lane] = run + incl - own;
-      run += __shfl_sync(0xffffffffu, incl, 31);
+  if (warp != 0) return;
+  // Exclusive prefix sums in place.
+  int64_t total = 0;
+  for (int b0 = 0; b0 < batch; b0 += 32) {
+    const int64_t own = b0 + lane < batch ? pref[b0 + lane] : 0;
+    int64_t incl = own;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
     }
-    __syncwarp();
-    const int64_t total = run;
-    const int64_t g0 = total * blockIdx.x / gridDim.x;
-    const int64_t g1 = total * (blockIdx.x + 1) / gridDim.x;
-    if (g1 > g0) {
-      // The largest b with pref[b] <= g0 (sequences without rows share their successor's start).
-      int lo = 0, hi = batch - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (pref[mid] <= g0) lo = mid;
-        else hi = mid - 1;
-      }
-      const Sequence s = load_sequence(a, lo);
-      const int64_t own = (lo + 1 < batch ? pref[lo + 1] : total) - pref[lo];
-      const int64_t per_head = own / a.cache.heads_kv;
-      int64_t rem = g0 - pref[lo];
-      const int hkv = static_cast<int>(rem / per_head);
-      rem -= hkv * per_head;
-      // The item that holds unit rem of this (sequence, head).
-      const int n = items_of(a, s);
-      int64_t before = 0;
-      int k = 0;
-      for (int k0 = 0; k0 < n; k0 += 32) {
-        const int64_t u = k0 + lane < n ? item_units(a, s, k0 + lane) : 0;
-        int64_t incl = u;
-        for (int o = 1; o < 32; o <<= 1) {
-          const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += v;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, before + incl > rem);
-        if (past != 0) {
-          const int at = __ffs(past) - 1;
-          before += __shfl_sync(0xffffffffu, incl - u, at);
-          k = k0 + at;
-          break;
-        }
-        before += __shfl_sync(0xffffffffu, incl, 31);
-      }
-      if (lane == 0) {
-        sh->b = lo;
-        sh->hkv = hkv;
-        sh->k = k;
-        sh->at = static_cast<int>(rem - before);
-      }
-    }
-    if (lane == 0) sh->units = g1 - g0;
+    if (b0 + lane < batch) pref[b0 + lane] = total + incl - own;
+    total += __shfl_sync(0xffffffffu, incl, 31);
   }
+  __syncwarp();
+  share_bounds(total, g0, g1);
+  if (g1 > g0) {
+    // The largest b with pref[b] <= g0 (sequences without rows share their successor's start).
+    int lo = 0, hi = batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pref[mid] <= g0) lo = mid;
+      else hi = mid - 1;
+    }
+    const int64_t own = (lo + 1 < batch ? pref[lo + 1] : total) - pref[lo];
+    locate_unit(a, sh, lo, load_sequence(a, lo), own, g0 - pref[lo], lane);
+  }
+  if (lane == 0) sh->units = g1 - g0;
 }
 
 // Four codes as two pairs of exact bf16 or fp16 values. fp16: the byte 128 + q in the low bits of
