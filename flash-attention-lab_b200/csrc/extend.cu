@@ -23,7 +23,7 @@
 //    its last row sees. When its tokens fit in one tile, both warpgroups work on that tile, on
 //    alternate key tiles (a chain of Q K^T, softmax, P V is latency bound: two of them per SM are
 //    twice the rate), and the first joins the two results through TMEM at the end.
-//  * One CTA per SM. The items' key tiles, in the order (sequence, KV head, item, key tile), are cut
+//  * One CTA per SM. The items' key tiles, in the order (KV head, sequence, item, key tile), are cut
 //    into equal shares (a tile of a two-tile item counts twice, and each item has a fixed part), so
 //    a long cache with few rows spreads over all SMs and ragged batches stay balanced. Every CTA
 //    finds its share from cu_seqlens and seq_lens on the device. An item that is cut leaves fp32

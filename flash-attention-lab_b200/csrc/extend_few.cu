@@ -4,7 +4,7 @@
 // memory straight into the registers of 16 x 8 x 16 warp MMAs instead of through 16-bit tiles (the
 // tcgen05 form of extend.cu took 297 us for 8 sequences of 24K keys, H_kv 8, D 128).
 //
-//  * One CTA per SM: one warp streams [128 keys x D] tiles of K and V codes by TMA, another turns the
+//  * One CTA per SM: two warps stream [128 keys x D] tiles of K and of V codes by TMA, one turns the
 //    keys' scales into what the scores need (below) beside them in the ring stage, and consumer
 //    warps take 16 keys of a tile each (two groups of eight warps on alternate tiles, or one),
 //    every warp with its own online softmax; their results are joined in a fixed order at the
@@ -40,9 +40,9 @@ struct FewGeometry {
   static constexpr int kRows = 8 * kBlocks;
   static constexpr int kGroups = 1;   // consumer groups, on alternate tiles
   static constexpr int kWarps = kGroups * kGroupWarps;
-  static constexpr int kCopyWarp = kWarps;               // TMA of the codes
-  static constexpr int kScaleWarp = kWarps + 1;
-  static constexpr int kThreads = (kWarps + 2) * 32;
+  static constexpr int kCopyWarp = kWarps;               // TMA of K, and kCopyWarp + 1 of V
+  static constexpr int kScaleWarp = kWarps + 2;
+  static constexpr int kThreads = (kWarps + 3) * 32;
   static constexpr int kTileBytes = kBN * D;             // K or V codes
   static constexpr int kStages = D == 128 ? 4 : 8;       // 128 KB of codes
   static constexpr int kScaleOffset = kStages * 2 * kTileBytes;
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
   if (threadIdx.x == 0) {
     sh->abort_flag = 0;
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&sh->full[i], 33);   // the TMA bytes and each lane's scales
+      mbar_init(&sh->full[i], 34);   // the bytes of K and of V, and each lane's scales
       mbar_init(&sh->empty[i], kGroupWarps);
     }
     fence_barrier_init();
@@ -199,13 +199,13 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
   Segment s;
   walk.start(a, sh->share);
 
-  if (warp == G::kCopyWarp) {
+  if (warp < G::kScaleWarp && warp >= G::kCopyWarp) {
     // ------------------------------- copies -------------------------------
-    // Lane i issues copy i of a tile: a part of box_rows rows, of K or of V.
-    const int parts = kBN / a.box_rows;
-    const bool issues = lane < 2 * parts;
-    const bool is_v = lane >= parts;
-    const int offset = (is_v ? lane - parts : lane) % parts * a.box_rows;   // of the part's keys
+    // Lane i issues copy i of a tile, a part of box_rows rows. Small pages are many copies, whose
+    // issue one warp for K and V could not keep up with (16-row pages: 2000 clocks per tile).
+    const bool is_v = warp != G::kCopyWarp;
+    const int offset = lane * a.box_rows;   // of the part's keys
+    const bool issues = offset < kBN;
     const bool paged = a.cache.block_tables != nullptr;
     const CUtensorMap* map = is_v ? &tmv : &tmk;
     const TmaCoords& c = is_v ? a.vc : a.kc;
@@ -220,14 +220,14 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
         if (paged) {
           const int page = a.cache.page.div(key);
           window.advance(a.cache, __shfl_sync(0xffffffffu, page, 0), lane);
-          blk = window.at(page);
+          blk = window.at(issues ? page : window.base);
           row = key - page * a.cache.page.d;
         }
         const int st = issued % kStages;
         ok = issued < kStages || mbar_wait(&sh->empty[st], ((issued / kStages) - 1) & 1, guard);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&sh->full[st], 2 * G::kTileBytes);
+        if (lane == 0) mbar_arrive_expect_tx(&sh->full[st], G::kTileBytes);
         __syncwarp();
         if (issues)
           tma_load_4d(smem + (2 * st + (is_v ? 1 : 0)) * G::kTileBytes + offset * D, map,

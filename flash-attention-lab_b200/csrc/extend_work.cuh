@@ -157,13 +157,14 @@ struct Walk {
         at = 0;
         if (++k >= items_of(a, seq)) {
           k = 0;
-          if (++hkv >= a.cache.heads_kv) {
-            hkv = 0;
-            if (left > 0) {
-              do {
-                seq = load_sequence(a, ++b);
-              } while (seq.n == 0);   // some later sequence has rows: units are left
-            }
+          if (left > 0) {
+            do {   // some later sequence has rows, or the next head's first: units are left
+              if (++b >= a.ragged.batch) {
+                b = 0;
+                ++hkv;
+              }
+              seq = load_sequence(a, b);
+            } while (seq.n == 0);
           }
         }
       }
@@ -199,12 +200,9 @@ __device__ __forceinline__ int64_t sequence_units(const ExtendArgs& a, const Seq
   return sum;
 }
 
-// The share's start: unit `rem` of sequence b, whose units over all heads are `own`. One warp.
-__device__ __forceinline__ void locate_unit(const ExtendArgs& a, Share* sh, int b, const Sequence& s,
-                                            int64_t own, int64_t rem, int lane) {
-  const int64_t per_head = divide(own, a.cache.heads_kv);
-  const int hkv = static_cast<int>(divide(rem, per_head));
-  rem -= hkv * per_head;
+// The share's start: unit `rem` of sequence b and head hkv. One warp.
+__device__ __forceinline__ void locate_unit(const ExtendArgs& a, Share* sh, int hkv, int b,
+                                            const Sequence& s, int64_t rem, int lane) {
   const int n = items_of(a, s);
   int64_t before = 0;
   int k = 0;
@@ -240,6 +238,9 @@ __device__ __forceinline__ void share_bounds(int64_t total, int64_t& g0, int64_t
   g1 = g0 + each + (c < more ? 1 : 0);
 }
 
+// The units of a call in the order (KV head, sequence, item, key tile): the CTAs that run together
+// read about the same keys of several heads, which share DRAM pages in a [.., H_kv, D] cache.
+//
 // Finds this CTA's share. All threads; `pref` is shared memory for batch values. It ends without a
 // barrier. Up to 32 sequences are one warp's work (a lane per sequence), which the start of a
 // short call waits for; more go through shared memory.
@@ -265,19 +266,20 @@ __device__ __forceinline__ void find_share(const ExtendArgs& a, Share* sh, int64
       const int64_t sum = sequence_units(a, t, lane);
       if (lane == b) own = sum;
     }
-    own *= a.cache.heads_kv;
     int64_t incl = own;
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    share_bounds(__shfl_sync(0xffffffffu, incl, 31), g0, g1);
+    const int64_t total = __shfl_sync(0xffffffffu, incl, 31);   // of one head
+    share_bounds(total * a.cache.heads_kv, g0, g1);
     if (g1 > g0) {
-      const int b = __ffs(__ballot_sync(0xffffffffu, incl > g0)) - 1;
+      const int hkv = static_cast<int>(divide(g0, total));
+      const int64_t rem = g0 - hkv * total;
+      const int b = __ffs(__ballot_sync(0xffffffffu, incl > rem)) - 1;
       const Sequence t{__shfl_sync(0xffffffffu, s.row0, b), __shfl_sync(0xffffffffu, s.n, b),
                        __shfl_sync(0xffffffffu, s.len, b)};
-      const int64_t units = __shfl_sync(0xffffffffu, own, b);
-      locate_unit(a, sh, b, t, units, g0 - (__shfl_sync(0xffffffffu, incl, b) - units), lane);
+      locate_unit(a, sh, hkv, b, t, rem - __shfl_sync(0xffffffffu, incl - own, b), lane);
     }
     if (lane == 0) sh->units = g1 - g0;
     return;
@@ -287,19 +289,19 @@ __device__ __forceinline__ void find_share(const ExtendArgs& a, Share* sh, int64
     const int n = items_of(a, s);
     int64_t sum = 0;
     for (int k = 0; k < min(n, kFew); ++k) sum += item_units(a, s, k);
-    pref[b] = n > kFew ? -1 : sum * a.cache.heads_kv;
+    pref[b] = n > kFew ? -1 : sum;
   }
   __syncthreads();
   for (int b = warp; b < batch; b += blockDim.x >> 5) {
     if (pref[b] != -1) continue;
     const int64_t sum = sequence_units(a, load_sequence(a, b), lane);
     __syncwarp();
-    if (lane == 0) pref[b] = sum * a.cache.heads_kv;
+    if (lane == 0) pref[b] = sum;
   }
   __syncthreads();
   if (warp != 0) return;
   // Exclusive prefix sums in place.
-  int64_t total = 0;
+  int64_t total = 0;   // of one head
   for (int b0 = 0; b0 < batch; b0 += 32) {
     const int64_t own = b0 + lane < batch ? pref[b0 + lane] : 0;
     int64_t incl = own;
@@ -311,17 +313,18 @@ __device__ __forceinline__ void find_share(const ExtendArgs& a, Share* sh, int64
     total += __shfl_sync(0xffffffffu, incl, 31);
   }
   __syncwarp();
-  share_bounds(total, g0, g1);
+  share_bounds(total * a.cache.heads_kv, g0, g1);
   if (g1 > g0) {
-    // The largest b with pref[b] <= g0 (sequences without rows share their successor's start).
+    const int hkv = static_cast<int>(divide(g0, total));
+    const int64_t rem = g0 - hkv * total;
+    // The largest b with pref[b] <= rem (sequences without rows share their successor's start).
     int lo = 0, hi = batch - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (pref[mid] <= g0) lo = mid;
+      if (pref[mid] <= rem) lo = mid;
       else hi = mid - 1;
     }
-    const int64_t own = (lo + 1 < batch ? pref[lo + 1] : total) - pref[lo];
-    locate_unit(a, sh, lo, load_sequence(a, lo), own, g0 - pref[lo], lane);
+    locate_unit(a, sh, hkv, lo, load_sequence(a, lo), rem - pref[lo], lane);
   }
   if (lane == 0) sh->units = g1 - g0;
 }

@@ -163,12 +163,17 @@ int encode_rows_map(CUtensorMap* map, TmaCoords* coords, const View4& v, int box
       : dtype == FLB_INT8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
       : dtype == FLB_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  // Rows of 8-bit codes are 128 or 64 bytes, and their neighbours in memory belong to other heads:
+  // a wider fetch into L2 reads those as well (1.4 x the bytes at H_kv 8, head_dim 128).
+  const CUtensorMapL2promotion promotion = dtype != FLB_INT8  ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                                           : v.size[3] >= 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                                              : CU_TENSOR_MAP_L2_PROMOTION_L2_64B;
   CUresult r = encode(map, type, 4, const_cast<void*>(v.base), dims, strides, box, elem_strides,
                       CU_TENSOR_MAP_INTERLEAVE_NONE,
                       swizzle == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
                      : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                                      : CU_TENSOR_MAP_SWIZZLE_NONE,
-                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                      promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     return fail(FLB_ERR_CUDA,
                 "cuTensorMapEncodeTiled failed (%d): dims %llu,%llu,%llu,%llu strides "
