@@ -12,11 +12,16 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <torch/csrc/autograd/python_variable.h>
+
 #include <cstdint>
+#include <initializer_list>
 #include <optional>
 #include <stdexcept>
 #include <string>
 #include <tuple>
+#include <unordered_map>
+#include <utility>
 
 #include "flash_lab_b200.h"
 
@@ -335,6 +340,170 @@ std::tuple<at::Tensor, at::Tensor> extend(const at::Tensor& q, const at::Tensor&
   return {o, lse};
 }
 
+// Eager calls whose metadata (shapes, strides, dtypes, devices and the arguments that the checks
+// read) passed flash_lab/kvcache.py's checks before go straight to the ops above: *_known() records a
+// call that passed, *_fast() runs a recorded one and returns None for any other. The checks depend
+// on nothing else, so every error still comes from Python, in its order.
+struct Known {
+  int64_t status = 0, sm_count = 0;
+};
+
+class KnownCalls {
+ public:
+  const Known* find(const std::string& key) const {
+    const auto it = calls_.find(key);
+    return it == calls_.end() ? nullptr : &it->second;
+  }
+  void add(std::string key, Known value) {
+    if (calls_.size() >= 4096) calls_.clear();   // many distinct shapes: start over, not grow
+    calls_[std::move(key)] = value;
+  }
+
+ private:
+  std::unordered_map<std::string, Known> calls_;   // under the GIL
+};
+
+KnownCalls g_known;
+
+template <typename V>
+void put(std::string& key, V value) {
+  key.append(reinterpret_cast<const char*>(&value), sizeof(value));
+}
+
+// Appends the metadata of plain tensors (or None); false for anything else.
+bool put_tensors(std::string& key, std::initializer_list<py::handle> tensors) {
+  for (const py::handle& h : tensors) {
+    if (h.is_none()) {
+      key.push_back('n');
+      continue;
+    }
+    if (!THPVariable_CheckExact(h.ptr())) return false;
+    const at::Tensor& t = THPVariable_Unpack(h.ptr());
+    key.push_back('t');
+    put(key, static_cast<int16_t>(t.scalar_type()));
+    put(key, static_cast<int16_t>(t.device().type()));
+    put(key, static_cast<int16_t>(t.device().index()));
+    put(key, static_cast<int16_t>(t.dim()));
+    for (int64_t n : t.sizes()) put(key, n);
+    for (int64_t n : t.strides()) put(key, n);
+  }
+  return true;
+}
+
+OptTensor optional_tensor(py::handle h) {
+  return h.is_none() ? OptTensor{} : OptTensor{THPVariable_Unpack(h.ptr())};
+}
+
+// Rows as the ops take them, [rows, H, D], and rows per sequence (0: from cu_seqlens).
+at::Tensor flat_rows(const at::Tensor& x, bool ragged, int64_t* per_seq) {
+  *per_seq = ragged ? 0 : x.dim() == 4 ? x.size(1) : 1;
+  return x.dim() == 4 ? x.flatten(0, 1) : x;
+}
+
+bool append_key(std::string& key, py::handle k, py::handle v, py::handle kc, py::handle vc,
+                py::handle lens, py::handle cu, py::handle tables, py::handle ks, py::handle vs) {
+  key.push_back('a');
+  return put_tensors(key, {k, v, kc, vc, lens, cu, tables, ks, vs});
+}
+
+void append_known(py::handle k, py::handle v, py::handle kc, py::handle vc, py::handle lens,
+                  py::handle cu, py::handle tables, py::handle ks, py::handle vs) {
+  std::string key;
+  if (append_key(key, k, v, kc, vc, lens, cu, tables, ks, vs)) g_known.add(std::move(key), {});
+}
+
+py::object append_fast(py::handle k, py::handle v, py::handle kc, py::handle vc, py::handle lens,
+                       py::handle cu, py::handle tables, py::handle ks, py::handle vs) {
+  std::string key;
+  if (!append_key(key, k, v, kc, vc, lens, cu, tables, ks, vs) || g_known.find(key) == nullptr)
+    return py::none();
+  int64_t per_seq = 0;
+  const at::Tensor k3 = flat_rows(THPVariable_Unpack(k.ptr()), !cu.is_none(), &per_seq);
+  const at::Tensor v3 = flat_rows(THPVariable_Unpack(v.ptr()), !cu.is_none(), &per_seq);
+  kv_append(k3, v3, THPVariable_Unpack(kc.ptr()), THPVariable_Unpack(vc.ptr()),
+            THPVariable_Unpack(lens.ptr()), optional_tensor(cu), optional_tensor(tables),
+            optional_tensor(ks), optional_tensor(vs), per_seq);
+  return py::bool_(true);
+}
+
+bool gather_key(std::string& key, py::handle kc, py::handle vc, py::handle lens, py::handle cu,
+                int64_t total, py::handle tables, py::handle ks, py::handle vs, int dtype) {
+  key.push_back('g');
+  put(key, total);
+  put(key, dtype);
+  return put_tensors(key, {kc, vc, lens, cu, tables, ks, vs});
+}
+
+int dtype_of(py::handle dtype) {   // -1: not given
+  return dtype.is_none() ? -1 : static_cast<int>(py::cast<at::ScalarType>(dtype));
+}
+
+void gather_known(py::handle kc, py::handle vc, py::handle lens, py::handle cu, int64_t total,
+                  py::handle tables, py::handle ks, py::handle vs, py::handle dtype) {
+  std::string key;
+  if (gather_key(key, kc, vc, lens, cu, total, tables, ks, vs, dtype_of(dtype)))
+    g_known.add(std::move(key), {});
+}
+
+py::object gather_fast(py::handle kc, py::handle vc, py::handle lens, py::handle cu, int64_t total,
+                       py::handle tables, py::handle ks, py::handle vs, py::handle dtype) {
+  std::string key;
+  const int code = dtype_of(dtype);
+  if (!gather_key(key, kc, vc, lens, cu, total, tables, ks, vs, code) ||
+      g_known.find(key) == nullptr)
+    return py::none();
+  const at::Tensor& k_cache = THPVariable_Unpack(kc.ptr());
+  const at::ScalarType own = k_cache.scalar_type();
+  const at::ScalarType out = code >= 0           ? static_cast<at::ScalarType>(code)
+                             : own == at::kChar ? at::kBFloat16
+                                                : own;
+  return py::cast(kv_gather(k_cache, THPVariable_Unpack(vc.ptr()), THPVariable_Unpack(lens.ptr()),
+                            THPVariable_Unpack(cu.ptr()), optional_tensor(tables),
+                            optional_tensor(ks), optional_tensor(vs), total, out));
+}
+
+// `entry` tells the callers of extend apart, whose checks differ.
+bool extend_key(std::string& key, int entry, py::handle q, py::handle kc, py::handle vc,
+                py::handle lens, py::handle cu, py::handle tables, py::handle ks, py::handle vs,
+                bool causal, double scale) {
+  key.push_back('e');
+  put(key, entry);
+  put(key, causal);
+  put(key, scale);
+  return put_tensors(key, {q, kc, vc, lens, cu, tables, ks, vs});
+}
+
+void extend_known(int entry, py::handle q, py::handle kc, py::handle vc, py::handle lens,
+                  py::handle cu, py::handle tables, py::handle ks, py::handle vs, bool causal,
+                  double scale, int64_t status, int64_t sm_count) {
+  std::string key;
+  if (extend_key(key, entry, q, kc, vc, lens, cu, tables, ks, vs, causal, scale))
+    g_known.add(std::move(key), {status, sm_count});
+}
+
+// o and lse in the shapes of q.
+py::object extend_fast(int entry, py::handle q, py::handle kc, py::handle vc, py::handle lens,
+                       py::handle cu, py::handle tables, py::handle ks, py::handle vs,
+                       bool causal, double scale) {
+  std::string key;
+  if (!extend_key(key, entry, q, kc, vc, lens, cu, tables, ks, vs, causal, scale))
+    return py::none();
+  const Known* known = g_known.find(key);
+  if (known == nullptr) return py::none();
+  const at::Tensor& rows = THPVariable_Unpack(q.ptr());
+  int64_t per_seq = 0;
+  const at::Tensor flat = flat_rows(rows, !cu.is_none(), &per_seq);
+  auto [o, lse] = extend(flat, THPVariable_Unpack(kc.ptr()), THPVariable_Unpack(vc.ptr()),
+                         THPVariable_Unpack(lens.ptr()), optional_tensor(cu),
+                         optional_tensor(tables), optional_tensor(ks), optional_tensor(vs), per_seq,
+                         causal, scale, known->status, known->sm_count);
+  if (rows.dim() == 4) {
+    o = o.view(rows.sizes());
+    lse = lse.view(rows.sizes().slice(0, 3));
+  }
+  return py::make_tuple(o, lse);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -344,5 +513,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_append", &kv_append, "writes rows into a KV cache (flb_kv_append)");
   m.def("kv_gather", &kv_gather, "k, v read back from a KV cache (flb_kv_gather)");
   m.def("extend", &extend, "o, lse of new tokens over a KV cache (flb_extend_fwd)");
+  m.def("append_known", &append_known);
+  m.def("append_fast", &append_fast, "kv_append of a call that passed the checks before, or None");
+  m.def("gather_known", &gather_known);
+  m.def("gather_fast", &gather_fast, "kv_gather of a call that passed the checks before, or None");
+  m.def("extend_known", &extend_known);
+  m.def("extend_fast", &extend_fast, "extend of a call that passed the checks before, or None");
   m.def("abi_version", &flb_version);
 }

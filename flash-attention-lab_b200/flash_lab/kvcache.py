@@ -171,29 +171,10 @@ def _check_head_dim(head_dim: int) -> None:
         raise ValueError(f"head_dim {head_dim} is not one of {_HEAD_DIMS}")
 
 
-# Arguments whose metadata passed the checks before (as ops._DECODE_CALLS): eager calls that differ
-# only in their data skip them.
-_CHECKED: dict[tuple, tuple] = {}
-
-
-def _meta(x):
-    if x is None:
-        return None
-    return (x.shape, x.stride(), x.dtype, x.device)
-
-
-def _checked(name, tensors, extra, check):
-    """check() memoised on the metadata of `tensors` (plain eager tensors only)."""
-    if not ops._plain_eager() or not all(x is None or type(x) is torch.Tensor for x in tensors):
-        return check()
-    key = (name, extra, *map(_meta, tensors))
-    hit = _CHECKED.get(key)
-    if hit is None:
-        hit = check()
-        if len(_CHECKED) >= 4096:   # many distinct shapes: start over rather than grow
-            _CHECKED.clear()
-        _CHECKED[key] = hit
-    return hit
+def _fast_binding():
+    """The PyTorch binding when a plain eager call may use its record of checked calls: calls with
+    the metadata of one that passed the checks below run without them (binding/torch_ops.cpp)."""
+    return ops._NATIVE if ops._NATIVE is not None and not ops.DEBUG and ops._plain_eager() else None
 
 
 def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -208,31 +189,30 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     lies outside the cache, whose page is not a block of the pool, or that belong to no sequence
     are skipped. Two rows that name the same cache row race.
     """
-    def check():
-        shape = check_cache_inputs(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale,
-                                   cu_seqlens, {"k": k, "v": v})
-        if k.shape != v.shape:
-            raise ValueError(f"k and v must have the same shape, got {tuple(k.shape)} and "
-                             f"{tuple(v.shape)}")
-        if k.dtype != v.dtype or k.dtype not in _ROW_DTYPES or \
-                not (shape.int8 or k.dtype == k_cache.dtype):
-            raise TypeError(f"k and v must share the cache's dtype (any of {_ROW_DTYPES} for an "
-                            f"int8 cache), got {k.dtype}, {v.dtype} and {k_cache.dtype}")
-        rows, per_seq = ragged_rows("k", k, shape.batch, cu_seqlens)
-        ragged_rows("v", v, shape.batch, cu_seqlens)
-        if rows.shape[1:] != k_cache.shape[2:]:
-            raise ValueError(f"k and v rows are {tuple(rows.shape[1:])} (heads, head_dim), the "
-                             f"cache's {tuple(k_cache.shape[2:])}")
-        _check_head_dim(shape.head_dim)
-        _require_kernels(k.device)
-        return (per_seq,)
-
-    (per_seq,) = _checked("append", (k, v, k_cache, v_cache, seq_lens, cu_seqlens, block_tables,
-                                     k_scale, v_scale), None, check)
-    if k.dim() == 4:
-        k, v = k.flatten(0, 1), v.flatten(0, 1)
-    ops._call_op("kv_append", k, v, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scale,
+    args = (k, v, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scale, v_scale)
+    fast = _fast_binding()
+    if fast is not None and fast.append_fast(*args):
+        return
+    shape = check_cache_inputs(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale,
+                               cu_seqlens, {"k": k, "v": v})
+    if k.shape != v.shape:
+        raise ValueError(f"k and v must have the same shape, got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    if k.dtype != v.dtype or k.dtype not in _ROW_DTYPES or \
+            not (shape.int8 or k.dtype == k_cache.dtype):
+        raise TypeError(f"k and v must share the cache's dtype (any of {_ROW_DTYPES} for an "
+                        f"int8 cache), got {k.dtype}, {v.dtype} and {k_cache.dtype}")
+    k3, per_seq = ragged_rows("k", k, shape.batch, cu_seqlens)
+    v3, _ = ragged_rows("v", v, shape.batch, cu_seqlens)
+    if k3.shape[1:] != k_cache.shape[2:]:
+        raise ValueError(f"k and v rows are {tuple(k3.shape[1:])} (heads, head_dim), the "
+                         f"cache's {tuple(k_cache.shape[2:])}")
+    _check_head_dim(shape.head_dim)
+    _require_kernels(k.device)
+    ops._call_op("kv_append", k3, v3, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scale,
                  v_scale, per_seq)
+    if fast is not None:
+        fast.append_known(*args)
 
 
 def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, seq_lens: torch.Tensor,
@@ -246,25 +226,28 @@ def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, seq_lens: torch.Tens
     give zeros. `total` (host int) is the number of rows to return, cu_seqlens[B] or more. An int8
     cache is read back as `dtype` (bf16 unless given); any other cache has its own dtype.
     """
-    def check():
-        shape = check_cache_inputs(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale,
-                                   cu_seqlens)
-        if cu_seqlens is None:
-            raise TypeError("cu_seqlens must be a torch.Tensor, got NoneType")
-        if total < 1:
-            raise ValueError(f"total must be positive, got {total}")
-        out = dtype if dtype is not None else torch.bfloat16 if shape.int8 else k_cache.dtype
-        if out not in _ROW_DTYPES or not (shape.int8 or out == k_cache.dtype):
-            raise TypeError(f"dtype must be the cache's own (any of {_ROW_DTYPES} for an int8 "
-                            f"cache), got {out} and {k_cache.dtype}")
-        _check_head_dim(shape.head_dim)
-        _require_kernels(k_cache.device)
-        return (out,)
-
-    (out,) = _checked("gather", (k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scale,
-                                 v_scale), (total, dtype), check)
-    return ops._call_op("kv_gather", k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scale,
+    args = (k_cache, v_cache, seq_lens, cu_seqlens, total, block_tables, k_scale, v_scale, dtype)
+    fast = _fast_binding() if isinstance(total, int) else None
+    if fast is not None:
+        done = fast.gather_fast(*args)
+        if done is not None:
+            return done
+    shape = check_cache_inputs(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale, cu_seqlens)
+    if cu_seqlens is None:
+        raise TypeError("cu_seqlens must be a torch.Tensor, got NoneType")
+    if total < 1:
+        raise ValueError(f"total must be positive, got {total}")
+    out = dtype if dtype is not None else torch.bfloat16 if shape.int8 else k_cache.dtype
+    if out not in _ROW_DTYPES or not (shape.int8 or out == k_cache.dtype):
+        raise TypeError(f"dtype must be the cache's own (any of {_ROW_DTYPES} for an int8 "
+                        f"cache), got {out} and {k_cache.dtype}")
+    _check_head_dim(shape.head_dim)
+    _require_kernels(k_cache.device)
+    done = ops._call_op("kv_gather", k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scale,
                         v_scale, total, out)
+    if fast is not None:
+        fast.gather_known(*args)
+    return done
 
 
 def extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seq_lens: torch.Tensor,
@@ -289,49 +272,58 @@ def extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seq_le
     causal mask keeps from that key (int8 caches: only for the rows that see it); keys at or past
     seq_lens[b] are never read into a result.
     """
+    out, lse = _extend_checked(0, q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, causal,
+                               softmax_scale, k_scale, v_scale)
+    return (out, lse) if return_lse else out
+
+
+def _extend_checked(entry, q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, causal,
+                    softmax_scale, k_scale, v_scale):
+    """extend (entry 0) and decode over an int8 cache (entry 1): o and lse in q's shapes."""
     _require_tensor("q", q)
+    if entry == 1 and q.dim() == 4 and q.shape[1] != 1:
+        raise ValueError(f"decode takes one query token per sequence, got q {tuple(q.shape)}")
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(max(q.shape[-1], 1))
-
-    def check():
-        shape = check_cache_inputs(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale,
-                                   cu_seqlens, {"q": q})
-        if q.dtype not in _HALF or not (shape.int8 or q.dtype == k_cache.dtype):
-            raise TypeError(f"q must be one of {_HALF} and the cache q's dtype or int8, got "
-                            f"{q.dtype} and {k_cache.dtype}")
-        rows, per_seq = ragged_rows("q", q, shape.batch, cu_seqlens)
-        if rows.shape[2] != shape.head_dim:
-            raise ValueError(f"head_dim mismatch: q has {rows.shape[2]}, the cache has "
-                             f"{shape.head_dim}")
-        _check_heads(rows.shape[1], shape.heads_kv)
-        if rows.shape[1] // shape.heads_kv > _MAX_GROUP:
-            raise ValueError(f"at most {_MAX_GROUP} query heads per KV head, got "
-                             f"{rows.shape[1]} and {shape.heads_kv}")
-        if shape.page_size and not (shape.page_size in (8, 16, 32) or shape.page_size % 64 == 0):
-            raise ValueError(f"page_size {shape.page_size} is not 8, 16, 32 or a multiple of 64")
-        if not (scale > 0 and math.isfinite(scale)):
-            raise ValueError(f"softmax_scale must be positive, got {scale}")
-        _check_head_dim(shape.head_dim)
-        _require_kernels(q.device)
-        return (per_seq,)
-
-    (per_seq,) = _checked("extend", (q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables,
-                                     k_scale, v_scale), scale, check)
-    q3 = q.flatten(0, 1) if q.dim() == 4 else q
+    causal = bool(causal)
+    args = (q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scale, v_scale, causal, scale)
+    fast = _fast_binding()
+    if fast is not None:
+        done = fast.extend_fast(entry, *args)
+        if done is not None:
+            return done
+    shape = check_cache_inputs(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale,
+                               cu_seqlens, {"q": q})
+    if q.dtype not in _HALF or not (shape.int8 or q.dtype == k_cache.dtype):
+        raise TypeError(f"q must be one of {_HALF} and the cache q's dtype or int8, got "
+                        f"{q.dtype} and {k_cache.dtype}")
+    q3, per_seq = ragged_rows("q", q, shape.batch, cu_seqlens)
+    if q3.shape[2] != shape.head_dim:
+        raise ValueError(f"head_dim mismatch: q has {q3.shape[2]}, the cache has {shape.head_dim}")
+    _check_heads(q3.shape[1], shape.heads_kv)
+    if q3.shape[1] // shape.heads_kv > _MAX_GROUP:
+        raise ValueError(f"at most {_MAX_GROUP} query heads per KV head, got "
+                         f"{q3.shape[1]} and {shape.heads_kv}")
+    if shape.page_size and not (shape.page_size in (8, 16, 32) or shape.page_size % 64 == 0):
+        raise ValueError(f"page_size {shape.page_size} is not 8, 16, 32 or a multiple of 64")
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"softmax_scale must be positive, got {scale}")
+    _check_head_dim(shape.head_dim)
+    _require_kernels(q.device)
     out, lse = ops._call_op("extend_sm100", q3, k_cache, v_cache, seq_lens, cu_seqlens,
                             block_tables, k_scale, v_scale, per_seq, causal, scale)
     if q.dim() == 4:
         out, lse = out.view(q.shape), lse.view(q.shape[:3])
-    return (out, lse) if return_lse else out
+    if fast is not None:
+        fast.extend_known(entry, *args, ops._status_ptr(q.device), ops._sm_count(q.device))
+    return out, lse
 
 
 def decode_int8(q, k_cache, v_cache, seq_lens, block_tables, softmax_scale, k_scale, v_scale,
                 return_lse: bool):
     """flash_lab.decode over an int8 cache: the one-row form of extend, with decode's shapes (q
     [B, 1, H, D] or [B, H, D], lse [B, H])."""
-    if isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[1] != 1:
-        raise ValueError(f"decode takes one query token per sequence, got q {tuple(q.shape)}")
-    out, lse = extend(q, k_cache, v_cache, seq_lens, None, block_tables, True, softmax_scale,
-                      k_scale, v_scale, return_lse=True)
+    out, lse = _extend_checked(1, q, k_cache, v_cache, seq_lens, None, block_tables, True,
+                               softmax_scale, k_scale, v_scale)
     if not return_lse:
         return out
     return out, lse.flatten(1) if q.dim() == 4 else lse
