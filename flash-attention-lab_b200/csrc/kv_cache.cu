@@ -3,15 +3,19 @@
 // sequences back as 16- or 32-bit rows).
 //
 // The mathematics. A row x of D values (one token, one KV head) is stored as q = round(x r),
-// r = min(127 / a, 2^100), a = max|x|, with the scale s = max(a / 127, 2^-100): |x - q s| is at most
-// half a step s plus the fp32 roundings of r, x r and s. The bounds keep r and s finite and normal
+// r = min(127 (1 / a), 2^100), a = max|x|, with the scale s = max(a (1 / 127), 2^-100): |x - q s| is at
+// most half a step s plus the fp32 roundings of 1 / a, r, x r and s. The bounds keep r and s finite and normal
 // for rows of zeros and denormals (and 127 s finite at the largest values). Non-finite rows are stored as (0, NaN).
 //
-// Both kernels move each byte once and do a handful of operations per value, so HBM bounds them
-// (launch latency for single-token calls). A warp handles one token and several of its 2 H_kv
-// (K or V, head) rows; 16 bytes of a row per lane, so a row is D * size / 16 lanes and its
-// maximum a shuffle reduction over them. The rows' loads are issued before the token's sequence
-// is looked up (append), which takes two or three dependent loads (offsets, length, block table).
+// Each byte moves once, so HBM should bound both directions (launch latency for single-token calls):
+// at 6.5 TB/s an SM has 15 values of a 16-bit row per clock, which leaves about eight instructions per
+// value and excludes the quarter-rate int <-> float conversions. Codes are rounded and read by
+// adding 1.5 2^23 or 2^23 instead, whose last place is 1. A lane holds 16 bytes of each half of an
+// outside row, so a row is D * size / 32 lanes and its maximum a shuffle reduction over them; with 16
+// bytes per lane and row the addresses cost more than the values. Finding where
+// a token lives takes three or four dependent loads (offsets, length, block table); one warp
+// does it for the block's tokens while the others' first rows are on their way (append), and
+// the rows then stream.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -19,6 +23,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "kv_cache.cuh"
 #include "sm100.cuh"
@@ -26,7 +31,12 @@
 namespace flb {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxTokens = 8;         // of one block (32: 5 % slower): a lane of its first warp finds
+                                      // each one's place
+constexpr int kBlocksAtLeast = 592;   // four per SM
+constexpr float kStep = 1.f / 127.f;
 constexpr float kMinScale = 0x1p-100f;
 constexpr float kMaxInverse = 0x1p+100f;
 constexpr float kMaxScale = 0x1.020406p+121f;   // the largest s with 127 s finite in fp32
@@ -39,204 +49,267 @@ struct RowsView {
   Ragged ragged;
 };
 
-// The 16-byte chunk of a row as floats (8 of a 16-bit type, 4 of fp32) and back.
+constexpr float kRoundBias = 12582912.f;   // 1.5 2^23: x + kRoundBias has round(x) in its low bits
+
+// The 16-byte chunk of a row as floats (8 of a 16-bit type, 4 of fp32).
 template <typename T>
 __device__ __forceinline__ void unpack16(const uint4& c, float (&x)[16 / sizeof(T)]) {
-  const T* e = reinterpret_cast<const T*>(&c);
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-  for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) x[i] = static_cast<float>(e[i]);
-}
-
-__device__ __forceinline__ uint32_t pack_codes(int a, int b, int c, int d) {
-  return (a & 0xff) | ((b & 0xff) << 8) | ((c & 0xff) << 16) | (static_cast<uint32_t>(d) << 24);
-}
-
-// Slot s of a token's 2 H_kv rows: the heads of K, then the heads of V.
-template <typename T, int D, bool kQuant, int kIter>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ KvView c,
-                                                             const __grid_constant__ RowsView r) {
-  constexpr int kPer = 16 / sizeof(T);          // values per lane
-  constexpr int kLanes = D / kPer;              // lanes per row
-  constexpr int kRows = 32 / kLanes;            // rows per warp and iteration
-  const int lane = threadIdx.x & 31;
-  const int sub = lane / kLanes, at = lane % kLanes;
-  const int slots = 2 * c.heads_kv;
-  const int warps_per_token = (slots + kRows * kIter - 1) / (kRows * kIter);
-  const int64_t w = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
-  const int64_t token = w / warps_per_token;
-  if (token >= r.ragged.rows) return;
-  const int t = static_cast<int>(token);
-  const int slot0 = static_cast<int>(w - token * warps_per_token) * (kRows * kIter);
-
-  uint4 in[kIter];
-#pragma unroll
-  for (int i = 0; i < kIter; ++i) {
-    const int slot = slot0 + i * kRows + sub;
-    const bool is_v = slot >= c.heads_kv;
-    const int h = is_v ? slot - c.heads_kv : slot;
-    in[i] = make_uint4(0, 0, 0, 0);
-    if (slot < slots) {
-      const int64_t off = is_v ? t * r.v_stride[0] + h * r.v_stride[1]
-                               : t * r.k_stride[0] + h * r.k_stride[1];
-      in[i] = __ldg(reinterpret_cast<const uint4*>(is_v ? r.v : r.k) +
-                    (off + at * kPer) / kPer);
-    }
-  }
-  int b, first, count;
-  if (!find_sequence(r.ragged, t, lane, b, first, count)) return;
-  int64_t outer, row;
-  if (!c.locate(b, __ldg(r.seq_lens + b) - count + (t - first), outer, row)) return;
-
-#pragma unroll
-  for (int i = 0; i < kIter; ++i) {
-    const int slot = slot0 + i * kRows + sub;
-    const bool is_v = slot >= c.heads_kv;
-    const int h = is_v ? slot - c.heads_kv : slot;
-    const int64_t* cs = is_v ? c.v_stride : c.k_stride;
-    const int64_t off = outer * cs[0] + row * cs[1] + h * cs[2] + at * kPer;
-    if constexpr (!kQuant) {
-      if (slot < slots) *reinterpret_cast<uint4*>(static_cast<T*>(is_v ? c.v : c.k) + off) = in[i];
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, float>::value) {
+      x[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     } else {
-      float x[kPer];
-      unpack16<T>(in[i], x);
-      // The largest magnitude as bits, where infinities and NaN exceed every finite value.
-      uint32_t top = 0;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float amax = __uint_as_float(top);
-      const bool finite = top < 0x7f800000u;
-      const float inv = fminf(__fdiv_rn(127.f, amax), kMaxInverse);
-      int q[kPer];
-#pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        q[e] = finite ? max(-127, min(127, __float2int_rn(__fmul_rn(x[e], inv)))) : 0;
-      if (slot < slots) {
-        int8_t* dst = static_cast<int8_t*>(is_v ? c.v : c.k) + off;
-        if constexpr (kPer == 8) {
-          *reinterpret_cast<uint2*>(dst) = make_uint2(pack_codes(q[0], q[1], q[2], q[3]),
-                                                      pack_codes(q[4], q[5], q[6], q[7]));
-        } else {
-          *reinterpret_cast<uint32_t*>(dst) = pack_codes(q[0], q[1], q[2], q[3]);
-        }
-        if (at == 0) {
-          const int64_t* ss = is_v ? c.vs_stride : c.ks_stride;
-          (is_v ? c.vs : c.ks)[outer * ss[0] + row * ss[1] + h * ss[2]] =
-              finite ? fminf(fmaxf(__fdiv_rn(amax, 127.f), kMinScale), kMaxScale)
-                     : __uint_as_float(0x7fffffffu);
-        }
-      }
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
     }
   }
 }
 
+// The largest magnitude of the chunk as the bits of a float, where infinities and NaN exceed every
+// finite value.
 template <typename T>
-__device__ __forceinline__ T from_float(float x) {
-  return static_cast<T>(x);
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
-  return __float2bfloat16_rn(x);
-}
-template <>
-__device__ __forceinline__ __half from_float<__half>(float x) {
-  return __float2half_rn(x);
-}
-
-template <typename T, int D, bool kQuant, int kIter>
-__global__ void __launch_bounds__(kThreads) kv_gather_kernel(const __grid_constant__ KvView c,
-                                                             const __grid_constant__ RowsView r) {
-  constexpr int kPer = 16 / sizeof(T);
-  constexpr int kLanes = D / kPer;
-  constexpr int kRows = 32 / kLanes;
-  const int lane = threadIdx.x & 31;
-  const int sub = lane / kLanes, at = lane % kLanes;
-  const int slots = 2 * c.heads_kv;
-  const int warps_per_token = (slots + kRows * kIter - 1) / (kRows * kIter);
-  const int64_t w = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
-  const int64_t token = w / warps_per_token;
-  if (token >= r.ragged.rows) return;
-  const int t = static_cast<int>(token);
-  const int slot0 = static_cast<int>(w - token * warps_per_token) * (kRows * kIter);
-
-  int b = 0, first = 0, count = 0;
-  int64_t outer = 0, row = 0;
-  const bool found = find_sequence(r.ragged, t, lane, b, first, count) &&
-                     t - first < __ldg(r.seq_lens + b) && c.locate(b, t - first, outer, row);
-  uint4 raw[kIter];
-  float scale[kIter];
+__device__ __forceinline__ uint32_t largest(const uint4& c) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  if constexpr (std::is_same<T, float>::value) {
+    return max(max(w[0] & 0x7fffffffu, w[1] & 0x7fffffffu),
+               max(w[2] & 0x7fffffffu, w[3] & 0x7fffffffu));
+  } else {
+    // NaN-propagating maxima of pairs.
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2,
+                                         __nv_bfloat162>::type;
+    T2 top = __habs2(*reinterpret_cast<const T2*>(&w[0]));
 #pragma unroll
-  for (int i = 0; i < kIter; ++i) {
-    const int slot = slot0 + i * kRows + sub;
-    const bool is_v = slot >= c.heads_kv;
-    const int h = is_v ? slot - c.heads_kv : slot;
-    raw[i] = make_uint4(0, 0, 0, 0);
-    scale[i] = 0.f;
-    if (found && slot < slots) {
-      const int64_t* cs = is_v ? c.v_stride : c.k_stride;
-      const int64_t off = outer * cs[0] + row * cs[1] + h * cs[2] + at * kPer;
-      const void* base = is_v ? c.v : c.k;
-      if constexpr (!kQuant) {
-        raw[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(base) + off);
-      } else {
-        const int8_t* src = static_cast<const int8_t*>(base) + off;
-        if constexpr (kPer == 8) {
-          const uint2 x = *reinterpret_cast<const uint2*>(src);
-          raw[i].x = x.x;
-          raw[i].y = x.y;
-        } else {
-          raw[i].x = *reinterpret_cast<const uint32_t*>(src);
+    for (int i = 1; i < 4; ++i) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const T2*>(&w[i])));
+    const float lo = static_cast<float>(top.x), hi = static_cast<float>(top.y);
+    return max(__float_as_uint(lo) & 0x7fffffffu, __float_as_uint(hi) & 0x7fffffffu);
+  }
+}
+
+// The codes round(x inv) of four values, in the bytes of a word.
+__device__ __forceinline__ uint32_t encode4(const float* x, float inv) {
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    b[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), kRoundBias));
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+
+// The values q s of the four codes of a word.
+__device__ __forceinline__ void decode4(uint32_t codes, float scale, float (&x)[4]) {
+  codes ^= 0x80808080u;   // 128 + q
+  // Bytes over the bits of 2^23: 2^23 + 128 + q.
+  const float f0 = __uint_as_float(__byte_perm(codes, 0x4b000000u, 0x7440));
+  const float f1 = __uint_as_float(__byte_perm(codes, 0x4b000000u, 0x7441));
+  const float f2 = __uint_as_float(__byte_perm(codes, 0x4b000000u, 0x7442));
+  const float f3 = __uint_as_float(__byte_perm(codes, 0x4b000000u, 0x7443));
+  fadd2(x[0], x[1], f0, f1, -8388736.f, -8388736.f);
+  fadd2(x[2], x[3], f2, f3, -8388736.f, -8388736.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] *= scale;
+}
+
+// A block moves the 2 H_kv rows (slots: the heads of K, then the heads of V) of `tokens` consecutive
+// tokens. kAppend: outside rows into the cache, else the cache into outside rows.
+template <typename T, int D, bool kQuant, bool kAppend>
+__global__ void __launch_bounds__(kThreads) kv_move_kernel(const __grid_constant__ KvView c,
+                                                           const __grid_constant__ RowsView r,
+                                                           const __grid_constant__ FastDiv slots,
+                                                           int tokens) {
+  constexpr int kPer = 16 / sizeof(T);          // values of 16 bytes
+  constexpr int kLanes = D / (2 * kPer);        // lanes per row: 16 bytes of each half
+  constexpr int kRows = 32 / kLanes;            // rows per warp and step
+  constexpr int kSteps = 2;                     // steps whose loads are issued together
+  // Where each token's rows are in the cache and in its scales (K, V, scales of K, of V); -1: nowhere.
+  __shared__ int64_t place[kMaxTokens][4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane / kLanes, at = lane % kLanes;
+  const int t0 = blockIdx.x * tokens;
+  const int rows = min(tokens, r.ragged.rows - t0) * slots.d;
+
+  struct Row {
+    int token, h;   // within the block; head
+    bool in, is_v;
+  };
+  auto row_at = [&](int step, int i) {
+    const int x = ((step * kSteps + i) * kWarps + warp) * kRows + sub;
+    Row row;
+    row.in = x < rows;
+    row.token = row.in ? slots.div(x) : 0;
+    const int slot = x - row.token * slots.d;
+    row.is_v = slot >= c.heads_kv;
+    row.h = row.is_v ? slot - c.heads_kv : slot;
+    return row;
+  };
+  struct Data {
+    uint4 half[2];
+    float scale;
+  };
+  auto outside = [&](const Row& x) {   // and D / 2 values on
+    const int64_t t = t0 + x.token;
+    return x.is_v ? reinterpret_cast<T*>(r.v) + t * r.v_stride[0] + x.h * r.v_stride[1] + at * kPer
+                  : reinterpret_cast<T*>(r.k) + t * r.k_stride[0] + x.h * r.k_stride[1] + at * kPer;
+  };
+  // A row as it comes: from outside (append), else codes or values of the cache.
+  auto load = [&](const Row& x) {
+    Data d;
+    d.half[0] = d.half[1] = make_uint4(0, 0, 0, 0);
+    d.scale = 0.f;
+    if constexpr (kAppend) {
+      if (x.in) {
+        const T* from = outside(x);
+        d.half[0] = __ldg(reinterpret_cast<const uint4*>(from));
+        d.half[1] = __ldg(reinterpret_cast<const uint4*>(from + D / 2));
+      }
+    } else {
+      const int64_t base = place[x.token][x.is_v];
+      if (x.in && base >= 0) {
+        const int64_t off = base + x.h * (x.is_v ? c.v_stride[2] : c.k_stride[2]) + at * kPer;
+        const void* from = x.is_v ? c.v : c.k;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if constexpr (!kQuant) {
+            d.half[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(from) + off +
+                                                        j * (D / 2));
+          } else {
+            const int8_t* src = static_cast<const int8_t*>(from) + off + j * (D / 2);
+            if constexpr (kPer == 8) {
+              const uint2 w = *reinterpret_cast<const uint2*>(src);
+              d.half[j].x = w.x;
+              d.half[j].y = w.y;
+            } else {
+              d.half[j].x = *reinterpret_cast<const uint32_t*>(src);
+            }
+          }
         }
-        const int64_t* ss = is_v ? c.vs_stride : c.ks_stride;
-        scale[i] = (is_v ? c.vs : c.ks)[outer * ss[0] + row * ss[1] + h * ss[2]];
+        if constexpr (kQuant)
+          d.scale = (x.is_v ? c.vs : c.ks)[place[x.token][2 + x.is_v] +
+                                           x.h * (x.is_v ? c.vs_stride[2] : c.ks_stride[2])];
       }
     }
-  }
+    return d;
+  };
+  auto store = [&](const Row& x, const Data& d) {
+    if constexpr (!kAppend) {
+      T* to = outside(x);
 #pragma unroll
-  for (int i = 0; i < kIter; ++i) {
-    const int slot = slot0 + i * kRows + sub;
-    if (slot >= slots) continue;
-    const bool is_v = slot >= c.heads_kv;
-    const int h = is_v ? slot - c.heads_kv : slot;
-    uint4 out = raw[i];
-    if constexpr (kQuant) {
-      const int8_t* q = reinterpret_cast<const int8_t*>(&raw[i]);
-      T* e = reinterpret_cast<T*>(&out);
+      for (int j = 0; j < 2; ++j) {
+        uint4 out = d.half[j];
+        if constexpr (kQuant) {
+          float y[4];
+          decode4(d.half[j].x, d.scale, y);
+          if constexpr (kPer == 8) {
+            float z[4];
+            decode4(d.half[j].y, d.scale, z);
+            out = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(z[0], z[1]),
+                             pack2<T>(z[2], z[3]));
+          } else {
+            out = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]),
+                             __float_as_uint(y[3]));
+          }
+        }
+        if (x.in) *reinterpret_cast<uint4*>(to + j * (D / 2)) = out;
+      }
+    } else {
+      const int64_t base = place[x.token][x.is_v];
+      const bool in = x.in && base >= 0;
+      const int64_t off = base + x.h * (x.is_v ? c.v_stride[2] : c.k_stride[2]) + at * kPer;
+      void* to = x.is_v ? c.v : c.k;
+      if constexpr (!kQuant) {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) e[j] = from_float<T>(static_cast<float>(q[j]) * scale[i]);
+        for (int j = 0; j < 2; ++j) {
+          if (in) *reinterpret_cast<uint4*>(static_cast<T*>(to) + off + j * (D / 2)) = d.half[j];
+        }
+      } else {
+        uint32_t top = max(largest<T>(d.half[0]), largest<T>(d.half[1]));
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1)
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float amax = __uint_as_float(top);
+        const bool finite = top < 0x7f800000u;
+        const float inv = fminf(__fmul_rn(127.f, __frcp_rn(amax)), kMaxInverse);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float y[kPer];
+          unpack16<T>(d.half[j], y);
+          uint32_t q[kPer / 4];
+#pragma unroll
+          for (int e = 0; e < kPer / 4; ++e) q[e] = finite ? encode4(y + 4 * e, inv) : 0u;
+          int8_t* dst = static_cast<int8_t*>(to) + off + j * (D / 2);
+          if (in) {
+            if constexpr (kPer == 8) {
+              *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
+            } else {
+              *reinterpret_cast<uint32_t*>(dst) = q[0];
+            }
+          }
+        }
+        if (in && at == 0)
+          (x.is_v ? c.vs : c.ks)[place[x.token][2 + x.is_v] +
+                                 x.h * (x.is_v ? c.vs_stride[2] : c.ks_stride[2])] =
+              finite ? fminf(fmaxf(__fmul_rn(amax, kStep), kMinScale), kMaxScale)
+                     : __uint_as_float(0x7fffffffu);
+      }
     }
-    const int64_t off = is_v ? t * r.v_stride[0] + h * r.v_stride[1]
-                             : t * r.k_stride[0] + h * r.k_stride[1];
-    *(reinterpret_cast<uint4*>(is_v ? r.v : r.k) + (off + at * kPer) / kPer) = out;
+  };
+
+  constexpr int kAtOnce = kSteps * kWarps * kRows;   // rows per round of the loop below
+  Row x[kSteps];
+  Data d[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    x[i] = row_at(0, i);
+    if (kAppend) d[i] = load(x[i]);   // does not depend on the places
+  }
+  if (warp == 0) {   // lanes past the block's tokens look up rows of the next one
+    int b, at_row, count;
+    int64_t outer = 0, row = 0;
+    const bool owned = find_sequences(r.ragged, t0, lane, b, at_row, count) && lane < tokens;
+    int pos = -1;
+    if (owned) {
+      const int len = __ldg(r.seq_lens + b);
+      pos = kAppend ? len - count + at_row : at_row < len ? at_row : -1;
+    }
+    const bool here = owned && c.locate(b, pos, outer, row);
+    if (lane < kMaxTokens) {
+      place[lane][0] = here ? outer * c.k_stride[0] + row * c.k_stride[1] : -1;
+      place[lane][1] = here ? outer * c.v_stride[0] + row * c.v_stride[1] : -1;
+      place[lane][2] = outer * c.ks_stride[0] + row * c.ks_stride[1];
+      place[lane][3] = outer * c.vs_stride[0] + row * c.vs_stride[1];
+    }
+  }
+  __syncthreads();
+  for (int step = 0; step * kAtOnce < rows; ++step) {
+    if (step > 0 || !kAppend) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        x[i] = row_at(step, i);
+        d[i] = load(x[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) store(x[i], d[i]);
   }
 }
-
-// Rows a warp handles per lane: one for calls of few tokens, whose latency is what counts (more
-// warps, each with one load), four for many (more bytes in flight per warp).
-constexpr int kManyTokens = 512;
 
 template <typename T, int D, bool kQuant>
 int launch(const KvView& c, const RowsView& r, bool append, cudaStream_t stream) {
-  constexpr int kRows = 32 / (D * static_cast<int>(sizeof(T)) / 16);
-  const int iter = r.ragged.rows >= kManyTokens ? 4 : 1;
-  const int per_token = (2 * c.heads_kv + kRows * iter - 1) / (kRows * iter);
-  const int64_t warps = static_cast<int64_t>(r.ragged.rows) * per_token;
-  const int64_t blocks = (warps * 32 + kThreads - 1) / kThreads;
-  if (blocks > 0x7fffffffLL) return fail(FLB_ERR_UNSUPPORTED, "problem too large for one launch");
-  const unsigned grid = static_cast<unsigned>(blocks);
-  if (append) {
-    if (iter == 4)
-      kv_append_kernel<T, D, kQuant, 4><<<grid, kThreads, 0, stream>>>(c, r);
-    else
-      kv_append_kernel<T, D, kQuant, 1><<<grid, kThreads, 0, stream>>>(c, r);
-    return check_cuda(cudaGetLastError(), "kv_append_kernel launch");
-  }
-  if (iter == 4)
-    kv_gather_kernel<T, D, kQuant, 4><<<grid, kThreads, 0, stream>>>(c, r);
+  // Tokens per block: as many as leave kBlocksAtLeast blocks, so that few tokens spread over the GPU
+  // and many share the look-up of their places.
+  int tokens = 1;
+  while (tokens < kMaxTokens && r.ragged.rows / (2 * tokens) >= kBlocksAtLeast) tokens *= 2;
+  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(r.ragged.rows) + tokens - 1) /
+                                              tokens);
+  const FastDiv slots = FastDiv::of(2 * c.heads_kv);
+  if (append)
+    kv_move_kernel<T, D, kQuant, true><<<grid, kThreads, 0, stream>>>(c, r, slots, tokens);
   else
-    kv_gather_kernel<T, D, kQuant, 1><<<grid, kThreads, 0, stream>>>(c, r);
-  return check_cuda(cudaGetLastError(), "kv_gather_kernel launch");
+    kv_move_kernel<T, D, kQuant, false><<<grid, kThreads, 0, stream>>>(c, r, slots, tokens);
+  return check_cuda(cudaGetLastError(), append ? "kv append launch" : "kv gather launch");
 }
 
 template <typename T>

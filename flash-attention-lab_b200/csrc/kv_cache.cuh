@@ -61,32 +61,39 @@ struct Ragged {
   int rows, rows_per_seq, batch;
 };
 
-// The sequence that owns row t and its first row and row count; false if none does. Called by
-// whole warps with one t. cu is searched 32 ways at once: one dependent load per factor of 32 of
-// the batch.
-__device__ __forceinline__ bool find_sequence(const Ragged& r, int t, int lane, int& b, int& first,
-                                              int& count) {
+// Where row t of a ragged call lives: the sequence b that owns it, its place in the sequence and
+// the sequence's row count; false if no sequence owns it. Lane i of a warp asks for row t0 + i.
+// cu is searched 32 ways at once for t0 (one dependent load per factor of 32 of the batch), and
+// from there each lane steps to its own row's sequence.
+__device__ __forceinline__ bool find_sequences(const Ragged& r, int t0, int lane, int& b, int& place,
+                                               int& count) {
+  const int t = t0 + lane;
   if (r.cu == nullptr) {
     b = t / r.rows_per_seq;
-    first = b * r.rows_per_seq;
+    place = t - b * r.rows_per_seq;
     count = r.rows_per_seq;
-    return b < r.batch;
+    return t < r.rows && b < r.batch;
   }
-  int lo = 0, hi = r.batch;   // the answer, if any, is the largest b in [lo, hi) with cu[b] <= t
+  int lo = 0, hi = r.batch;   // the largest b in [lo, hi) with cu[b] <= t0, or 0
   while (true) {
     const int step = (hi - lo + 31) / 32;
     const int i = lo + lane * step;
-    const bool below = i < hi && __ldg(r.cu + i) <= t;
-    const int n = __popc(__ballot_sync(0xffffffffu, below));
-    if (n == 0) return false;
+    const bool below = i < hi && __ldg(r.cu + i) <= t0;
+    const int n = max(__popc(__ballot_sync(0xffffffffu, below)), 1);
     lo += (n - 1) * step;
     hi = min(hi, lo + step);
     if (step == 1) break;
   }
   b = lo;
-  first = __ldg(r.cu + b);
-  count = __ldg(r.cu + b + 1) - first;
-  return t - first < count;
+  int first = __ldg(r.cu + b), end = __ldg(r.cu + b + 1);
+  while (t < r.rows && end <= t && b + 1 < r.batch) {
+    ++b;
+    first = end;
+    end = __ldg(r.cu + b + 1);
+  }
+  place = t - first;
+  count = end - first;
+  return t < r.rows && first <= t && t < end;
 }
 
 // Checks of an flb_kv_cache that do not depend on who uses it: required pointers, positive sizes,
