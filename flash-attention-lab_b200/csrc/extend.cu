@@ -82,7 +82,7 @@ struct Geometry {
   static constexpr int kOtherRegs = kInt8 ? 56 : 72;
   static_assert(2 * 128 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs <= kThreads * kLaunchRegs,
                 "the register split must fit in the launch's registers");
-  static_assert(kMaxBatch * 8 <= kSlots * kTileBytes, "prefix sums fit in the rings");
+  static_assert(kMaxBatch * 4 <= kSlots * kTileBytes, "prefix sums fit in the rings");
 };
 
 template <int kKSlots, int kVSlots, int kCodeSlots>
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     tmem_alloc(&sh->tmem_base, kTmemCols);
     tmem_relinquish();
   }
-  find_share(a, &sh->share, reinterpret_cast<int64_t*>(k_ring));
+  find_share(a, &sh->share, reinterpret_cast<int*>(k_ring));
   fence_proxy_async_shared();   // the rings were written here; TMA writes it next
   tc_fence_before();
   __syncthreads();
@@ -828,16 +828,17 @@ __global__ void __launch_bounds__(256) extend_merge_kernel(const __grid_constant
   const int cta = blockIdx.x;
   int open = -1;
   int4 meta = make_int4(0, 0, 0, 0);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int4 m = a.part_meta[2 * cta + i];
-    if ((m.x & (kPartValid | kPartOpens | kPartCloses)) == (kPartValid | kPartOpens)) {
-      open = 2 * cta + i;
-      meta = m;
-    }
+  const int4 m0 = a.part_meta[2 * cta], m1 = a.part_meta[2 * cta + 1];
+  for (int i = cta + 1 + threadIdx.x; i < ctas; i += 256) first_flags[i] = a.part_meta[2 * i].x;
+  constexpr int kWhich = kPartValid | kPartOpens | kPartCloses;
+  if ((m0.x & kWhich) == (kPartValid | kPartOpens)) {
+    open = 2 * cta;
+    meta = m0;
+  } else if ((m1.x & kWhich) == (kPartValid | kPartOpens)) {
+    open = 2 * cta + 1;
+    meta = m1;
   }
   if (open < 0) return;
-  for (int i = cta + 1 + threadIdx.x; i < ctas; i += 256) first_flags[i] = a.part_meta[2 * i].x;
   __syncthreads();
   const int idx = blockIdx.y * 256 + threadIdx.x;
   const int row = idx % a.part_rows, col = idx / a.part_rows;
@@ -861,7 +862,7 @@ __global__ void __launch_bounds__(256) extend_merge_kernel(const __grid_constant
     }
     return -1;
   };
-  constexpr int kBatch = 4;   // parts whose loads are issued together
+  constexpr int kBatch = 8;   // parts whose loads are issued together
   while (slot >= 0) {
     float2 ml[kBatch];
     float4 o0[kBatch], o1[kBatch];
@@ -1007,6 +1008,12 @@ int validate(const flb_kv_cache* c, const flb_extend_params* p) {
                 ps);
   if (c->batch > kMaxBatch)
     return fail(FLB_ERR_UNSUPPORTED, "more than %d sequences in one call", kMaxBatch);
+  // Units of one KV head (extend_work.cuh) must fit in 31 bits.
+  const int tile_tokens = kBM / (p->heads / c->heads_kv);
+  const int64_t items = p->rows / (2 * tile_tokens) + c->batch;
+  const int64_t max_units = items * (kItemUnits + 2 * ((c->max_seqlen + int64_t{kBN} - 1) / kBN));
+  if (max_units > 0x7fffffffLL)
+    return fail(FLB_ERR_UNSUPPORTED, "problem too large for one launch");
   const View4 qv{p->q, {1, p->rows, p->heads, c->head_dim},
                  {0, p->q_row_stride, p->q_head_stride, 1}, 2};
   const View4 ov{p->o, {1, p->rows, p->heads, c->head_dim},

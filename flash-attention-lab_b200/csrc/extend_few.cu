@@ -52,7 +52,7 @@ struct FewGeometry {
   static constexpr int kJoinOffset = kRawOffset + kRawTiles * 2 * kBN * 4;
   static constexpr int kJoinBytes = kWarps * kRows * (D + 2) * 4;
   static constexpr int kTailOffset = kJoinOffset + kJoinBytes;
-  static_assert(kMaxBatch * 8 <= kScaleOffset, "prefix sums fit in the ring");
+  static_assert(kMaxBatch * 4 <= kScaleOffset, "prefix sums fit in the ring");
 };
 
 template <int kStages>
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
   }
-  find_share(a, &sh->share, reinterpret_cast<int64_t*>(smem));
+  find_share(a, &sh->share, reinterpret_cast<int*>(smem));
   fence_proxy_async_shared();   // the ring was written here; TMA writes it next
   __syncthreads();
   const WaitGuard guard{reinterpret_cast<volatile int*>(&sh->abort_flag), a.status};

@@ -19,7 +19,7 @@ namespace flb {
 constexpr int kBN = 128;              // keys per tile
 constexpr float kRescaleThreshold = 8.0f;   // log2 units: weights stay <= 2^8
 constexpr int kItemUnits = 2;         // fixed cost of an item, in halves of a two-tile key tile
-constexpr int kMaxBatch = 8192;       // the units' prefix sums use the K/V ring before it fills
+constexpr int kMaxBatch = 16384;      // the units' prefix sums use the K/V ring before it fills
 constexpr float kMinScale = 0x1p-100f;
 constexpr int kMaxCtas = 256;         // SMs of a device (one CTA each)
 
@@ -191,28 +191,32 @@ __device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
                                                      static_cast<uint32_t>(y));
 }
 
+// Inclusive prefix sum over the lanes.
+__device__ __forceinline__ int prefix_sum(int x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += v;
+  }
+  return x;
+}
+
 // Units of a sequence's items of one KV head, by a whole warp.
-__device__ __forceinline__ int64_t sequence_units(const ExtendArgs& a, const Sequence& s, int lane) {
+__device__ __forceinline__ int sequence_units(const ExtendArgs& a, const Sequence& s, int lane) {
   const int n = items_of(a, s);
-  int64_t sum = 0;
+  int sum = 0;
   for (int k = lane; k < n; k += 32) sum += item_units(a, s, k);
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
+  return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(sum)));
 }
 
 // The share's start: unit `rem` of sequence b and head hkv. One warp.
 __device__ __forceinline__ void locate_unit(const ExtendArgs& a, Share* sh, int hkv, int b,
-                                            const Sequence& s, int64_t rem, int lane) {
+                                            const Sequence& s, int rem, int lane) {
   const int n = items_of(a, s);
-  int64_t before = 0;
-  int k = 0;
+  int before = 0, k = 0;
   for (int k0 = 0; n > 1 && k0 < n; k0 += 32) {
-    const int64_t u = k0 + lane < n ? item_units(a, s, k0 + lane) : 0;
-    int64_t incl = u;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
+    const int u = k0 + lane < n ? item_units(a, s, k0 + lane) : 0;
+    const int incl = prefix_sum(u, lane);
     const uint32_t past = __ballot_sync(0xffffffffu, before + incl > rem);
     if (past != 0) {
       const int at = __ffs(past) - 1;
@@ -226,7 +230,7 @@ __device__ __forceinline__ void locate_unit(const ExtendArgs& a, Share* sh, int 
     sh->b = b;
     sh->hkv = hkv;
     sh->k = k;
-    sh->at = static_cast<int>(rem - before);
+    sh->at = rem - before;
   }
 }
 
@@ -240,11 +244,12 @@ __device__ __forceinline__ void share_bounds(int64_t total, int64_t& g0, int64_t
 
 // The units of a call in the order (KV head, sequence, item, key tile): the CTAs that run together
 // read about the same keys of several heads, which share DRAM pages in a [.., H_kv, D] cache.
+// Those of one head fit in 31 bits (max_units bounds them on the host).
 //
 // Finds this CTA's share. All threads; `pref` is shared memory for batch values. It ends without a
 // barrier. Up to 32 sequences are one warp's work (a lane per sequence), which the start of a
 // short call waits for; more go through shared memory.
-__device__ __forceinline__ void find_share(const ExtendArgs& a, Share* sh, int64_t* pref) {
+__device__ __forceinline__ void find_share(const ExtendArgs& a, Share* sh, int* pref) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int batch = a.ragged.batch;
   constexpr int kFew = 4;   // items one thread sums by itself
@@ -254,32 +259,29 @@ __device__ __forceinline__ void find_share(const ExtendArgs& a, Share* sh, int64
     Sequence s{0, 0, 0};
     if (lane < batch) s = load_sequence(a, lane);
     const int n = items_of(a, s);
-    int64_t own = 0;
+    int own = 0;
     if (n <= kFew) {
       for (int k = 0; k < n; ++k) own += item_units(a, s, k);
     }
+    auto sequence_of = [&](int b) {
+      return Sequence{__shfl_sync(0xffffffffu, s.row0, b), __shfl_sync(0xffffffffu, s.n, b),
+                      __shfl_sync(0xffffffffu, s.len, b)};
+    };
     for (uint32_t long_ones = __ballot_sync(0xffffffffu, n > kFew); long_ones != 0;
          long_ones &= long_ones - 1) {
       const int b = __ffs(long_ones) - 1;
-      const Sequence t{__shfl_sync(0xffffffffu, s.row0, b), __shfl_sync(0xffffffffu, s.n, b),
-                       __shfl_sync(0xffffffffu, s.len, b)};
-      const int64_t sum = sequence_units(a, t, lane);
+      const int sum = sequence_units(a, sequence_of(b), lane);
       if (lane == b) own = sum;
     }
-    int64_t incl = own;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    const int64_t total = __shfl_sync(0xffffffffu, incl, 31);   // of one head
-    share_bounds(total * a.cache.heads_kv, g0, g1);
+    const int incl = prefix_sum(own, lane);
+    const int total = __shfl_sync(0xffffffffu, incl, 31);   // of one head
+    share_bounds(static_cast<int64_t>(total) * a.cache.heads_kv, g0, g1);
     if (g1 > g0) {
       const int hkv = static_cast<int>(divide(g0, total));
-      const int64_t rem = g0 - hkv * total;
+      const int rem = static_cast<int>(g0 - static_cast<int64_t>(hkv) * total);
       const int b = __ffs(__ballot_sync(0xffffffffu, incl > rem)) - 1;
-      const Sequence t{__shfl_sync(0xffffffffu, s.row0, b), __shfl_sync(0xffffffffu, s.n, b),
-                       __shfl_sync(0xffffffffu, s.len, b)};
-      locate_unit(a, sh, hkv, b, t, rem - __shfl_sync(0xffffffffu, incl - own, b), lane);
+      locate_unit(a, sh, hkv, b, sequence_of(b), rem - __shfl_sync(0xffffffffu, incl - own, b),
+                  lane);
     }
     if (lane == 0) sh->units = g1 - g0;
     return;
@@ -287,36 +289,32 @@ __device__ __forceinline__ void find_share(const ExtendArgs& a, Share* sh, int64
   for (int b = threadIdx.x; b < batch; b += blockDim.x) {
     const Sequence s = load_sequence(a, b);
     const int n = items_of(a, s);
-    int64_t sum = 0;
+    int sum = 0;
     for (int k = 0; k < min(n, kFew); ++k) sum += item_units(a, s, k);
     pref[b] = n > kFew ? -1 : sum;
   }
   __syncthreads();
   for (int b = warp; b < batch; b += blockDim.x >> 5) {
     if (pref[b] != -1) continue;
-    const int64_t sum = sequence_units(a, load_sequence(a, b), lane);
+    const int sum = sequence_units(a, load_sequence(a, b), lane);
     __syncwarp();
     if (lane == 0) pref[b] = sum;
   }
   __syncthreads();
   if (warp != 0) return;
   // Exclusive prefix sums in place.
-  int64_t total = 0;   // of one head
+  int total = 0;   // of one head
   for (int b0 = 0; b0 < batch; b0 += 32) {
-    const int64_t own = b0 + lane < batch ? pref[b0 + lane] : 0;
-    int64_t incl = own;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
+    const int own = b0 + lane < batch ? pref[b0 + lane] : 0;
+    const int incl = prefix_sum(own, lane);
     if (b0 + lane < batch) pref[b0 + lane] = total + incl - own;
     total += __shfl_sync(0xffffffffu, incl, 31);
   }
   __syncwarp();
-  share_bounds(total * a.cache.heads_kv, g0, g1);
+  share_bounds(static_cast<int64_t>(total) * a.cache.heads_kv, g0, g1);
   if (g1 > g0) {
     const int hkv = static_cast<int>(divide(g0, total));
-    const int64_t rem = g0 - hkv * total;
+    const int rem = static_cast<int>(g0 - static_cast<int64_t>(hkv) * total);
     // The largest b with pref[b] <= rem (sequences without rows share their successor's start).
     int lo = 0, hi = batch - 1;
     while (lo < hi) {

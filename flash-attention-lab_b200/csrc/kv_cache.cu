@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const __grid_constant
   constexpr int kPer = 16 / sizeof(T);          // values of 16 bytes
   constexpr int kLanes = D / (2 * kPer);        // lanes per row: 16 bytes of each half
   constexpr int kRows = 32 / kLanes;            // rows per warp and step
-  constexpr int kSteps = 2;                     // steps whose loads are issued together
+  constexpr int kSteps = kQuant ? 2 : 4;        // steps whose loads are issued together
   // Where each token's rows are in the cache and in its scales (K, V, scales of K, of V); -1: nowhere.
   __shared__ int64_t place[kMaxTokens][4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
