@@ -50,11 +50,10 @@ namespace {
 constexpr int kBM = 128;              // score rows per tile
 constexpr int kBoxBytes = kBM * 128;  // a swizzled [128 rows x 64 columns] 16-bit box
 constexpr uint32_t kTmemCols = 512;   // S0 | S1 | O0 | O1
-constexpr int kScaleSlots = 4;        // key tiles whose scales are held (see the converter)
 
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
-constexpr int kConvertWarp = 12;      // int8: warps 12-15
+constexpr int kConvertWarp = 12;      // int8: warps 12-15 (K and scales), 16-19 (V)
 
 // 16-bit: 128 KB of K/V tiles beside the two Q tiles. int8: 96 KB of 16-bit tiles, 48 KB of codes
 // (what is in flight from HBM). K and V have rings of their own, and K runs one tile ahead of V:
@@ -70,22 +69,25 @@ struct Geometry {
   static constexpr int kVSlots = (kInt8 ? 1 : 2) * (128 / D);
   static constexpr int kSlots = kKSlots + kVSlots;
   static constexpr int kCodeSlots = kInt8 ? 3 * (128 / D) : 0;
-  static constexpr int kScaleBytes = kInt8 ? kScaleSlots * 3 * kBN * 4 : 0;
+  // Key tiles whose scales are held: a K tile is converted once Q K^T of the tile kKSlots earlier
+  // has been issued, which follows the softmax of tiles two or more before that one.
+  static constexpr int kScaleSlots = kInt8 ? kKSlots + 2 : 0;
+  static constexpr int kScaleBytes = kScaleSlots * 3 * kBN * 4;
   static constexpr int kRingOffset = 2 * kTileBytes;
   static constexpr int kCodeOffset = kRingOffset + kSlots * kTileBytes;
   static constexpr int kScaleOffset = kCodeOffset + kCodeSlots * kCodeBytes;
   static constexpr int kTailOffset = kScaleOffset + kScaleBytes;
-  static constexpr int kThreads = kInt8 ? 512 : 384;
+  static constexpr int kThreads = kInt8 ? 640 : 384;
   // The register split (setmaxnreg) must not exceed what the CTA is launched with.
-  static constexpr int kLaunchRegs = kInt8 ? 128 : 168;
-  static constexpr int kSoftmaxRegs = kInt8 ? 200 : 216;
-  static constexpr int kOtherRegs = kInt8 ? 56 : 72;
+  static constexpr int kLaunchRegs = kInt8 ? 96 : 168;
+  static constexpr int kSoftmaxRegs = kInt8 ? 128 : 216;
+  static constexpr int kOtherRegs = kInt8 ? 72 : 72;
   static_assert(2 * 128 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs <= kThreads * kLaunchRegs,
                 "the register split must fit in the launch's registers");
   static_assert(kMaxBatch * 4 <= kSlots * kTileBytes, "prefix sums fit in the rings");
 };
 
-template <int kKSlots, int kVSlots, int kCodeSlots>
+template <int kKSlots, int kVSlots, int kCodeSlots, int kScaleSlots>
 struct Shared {
   uint64_t q_full[2];
   uint64_t q_free[2];        // the last Q K^T of an item that reads a Q tile has completed
@@ -95,7 +97,7 @@ struct Shared {
   uint64_t v_empty[kVSlots];
   uint64_t code_full[kCodeSlots + 1];
   uint64_t code_empty[kCodeSlots + 1];
-  uint64_t scale_full[kScaleSlots];
+  uint64_t scale_full[kScaleSlots + 1];
   uint64_t s_full[2];
   uint64_t p_half[2][2];     // P of keys 0-63 / 64-127 of a tile stored in TMEM
   uint64_t o_full[2];
@@ -164,39 +166,149 @@ __device__ __forceinline__ void convert_tile(const uint8_t* codes, uint8_t* tile
 // Softmax
 // --------------------------------------------------------------------------------------------
 
-// 2^x of a row's 128 scores, row sums in ps, P packed to 16 bits in TMEM columns [0, 64) of the
-// row's S region, published in two halves of 64 keys. x = s sl2 + nref (16-bit caches), or
-// z + nref with the sum weighted by 1 / sv (int8: rsv).
-template <typename P, bool kInt8>
-__device__ __forceinline__ void exp_store(const float* sf, float sl2, float nref, const float* rsv,
-                                          float (&ps)[4], uint32_t taddr_s, uint64_t* bars) {
+// The reference point of a row moves only when its maximum mt (log2 domain) passes it by more than
+// 2^8; the row sum and O (in TMEM) follow. P V of the chain's previous step has completed (the
+// scores depend on it) and this step's waits for the first half of P.
+template <int D>
+__device__ __forceinline__ void move_reference(float mt, float& m_ref, float& l_sum,
+                                               uint32_t taddr_o) {
+  float m_new = m_ref;
+  if (m_ref == -INFINITY || mt > m_ref + kRescaleThreshold) m_new = fmaxf(m_ref, mt);
+  const bool rescale = (m_new != m_ref) && (m_ref != -INFINITY);
+  const float factor = rescale ? ex2(m_ref - m_new) : 1.f;
+  if (rescale) l_sum *= factor;
+  m_ref = m_new;
+  if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+    for (int i = 0; i < D / 16; ++i) {
+      uint32_t ov[16];
+      tmem_ld16(taddr_o + i * 16, ov);
+      tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * factor);
+      tmem_st16(taddr_o + i * 16, ov);
+    }
+  }
+}
+
+// Publishes one half of P (64 keys) to the MMA warp.
+__device__ __forceinline__ void publish_half(uint64_t* bar) {
+  tmem_st_wait();
+  tc_fence_before();
+  mbar_arrive(bar);
+}
+
+// One key tile of one score row of a 16-bit cache: scores in 128 TMEM columns, keys at or past
+// `visible` hidden when `masked`; P as packed pairs over the first 64 columns.
+template <typename T, int D>
+__device__ __forceinline__ void softmax_tile(uint32_t taddr_s, uint32_t taddr_o, float sl2,
+                                             bool masked, int visible, float& m_ref, float& l_sum,
+                                             uint64_t* bars) {
+  uint32_t sr[128];
+#pragma unroll
+  for (int i = 0; i < 128; i += 32)
+    tmem_ld32(taddr_s + i, *reinterpret_cast<uint32_t(*)[32]>(&sr[i]));
+  tmem_ld_wait();
+  float* sf = reinterpret_cast<float*>(sr);
+  if (masked) {
+#pragma unroll
+    for (int i = 0; i < 128; ++i) {
+      if (i >= visible) sf[i] = -INFINITY;
+    }
+  }
+  float mx8[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mx8[i] = fmaxf(sf[i], sf[i + 8]);
+#pragma unroll
+  for (int i0 = 16; i0 < 128; i0 += 16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx8[i] = fmax3(mx8[i], sf[i0 + 2 * i], sf[i0 + 2 * i + 1]);
+  }
+  const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]),
+                         fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+  move_reference<D>(mx == -INFINITY ? -INFINITY : mx * sl2, m_ref, l_sum, taddr_o);
+  const float nref = m_ref == -INFINITY ? 0.f : -m_ref;
+  float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     uint32_t pk[32];
 #pragma unroll
     for (int c = 0; c < 32; ++c) {
-      const int i = half * 64 + 2 * c;
+      const int i = half * 64 + 2 * c, acc = (c & 1) * 2;
       float x0, x1;
-      if constexpr (kInt8) {
-        fadd2(x0, x1, sf[i], sf[i + 1], nref, nref);
-      } else {
-        ffma2(x0, x1, sf[i], sf[i + 1], sl2, sl2, nref, nref);
-      }
+      ffma2(x0, x1, sf[i], sf[i + 1], sl2, sl2, nref, nref);
       const float p0 = ex2(x0), p1 = ex2(x1);
-      const int acc = (c & 1) * 2;
-      if constexpr (kInt8) {
-        const float2 r = *reinterpret_cast<const float2*>(rsv + i);
-        ffma2(ps[acc], ps[acc + 1], p0, p1, r.x, r.y, ps[acc], ps[acc + 1]);
-      } else {
-        fadd2(ps[acc], ps[acc + 1], ps[acc], ps[acc + 1], p0, p1);
-      }
-      pk[c] = pack2<P>(p0, p1);
+      fadd2(ps[acc], ps[acc + 1], ps[acc], ps[acc + 1], p0, p1);
+      pk[c] = pack2<T>(p0, p1);
     }
     tmem_st32(taddr_s + half * 32, pk);
-    tmem_st_wait();
-    tc_fence_before();
-    mbar_arrive(&bars[half]);
+    publish_half(&bars[half]);
   }
+  l_sum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+}
+
+// The same over an int8 cache, with fp16 weights. `scales` holds the tile's per-key numbers in shared
+// memory: mult, log2 sv and 1 / sv. They are read once: the scaled scores z go back to TMEM between
+// the two passes. 32 columns at a time leave registers to read ahead; with all 128 in registers the
+// loop spilled, and the spills cost more than the softmax.
+template <int D>
+__device__ __forceinline__ void softmax_tile_int8(uint32_t taddr_s, uint32_t taddr_o,
+                                                  const float* scales, bool masked, int visible,
+                                                  float& m_ref, float& l_sum, uint64_t* bars) {
+  float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+  for (int c0 = 0; c0 < 128; c0 += 32) {
+    uint32_t sr[32];
+    tmem_ld32(taddr_s + c0, sr);
+    tmem_ld_wait();
+    float* z = reinterpret_cast<float*>(sr);
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      const float4 mul = *reinterpret_cast<const float4*>(scales + c0 + i);
+      const float4 add = *reinterpret_cast<const float4*>(scales + kBN + c0 + i);
+      ffma2(z[i], z[i + 1], z[i], z[i + 1], mul.x, mul.y, add.x, add.y);
+      ffma2(z[i + 2], z[i + 3], z[i + 2], z[i + 3], mul.z, mul.w, add.z, add.w);
+    }
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        if (c0 + i >= visible) z[i] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx4[e] = fmax3(mx4[e], z[i + 2 * e], z[i + 2 * e + 1]);
+    }
+    tmem_st32(taddr_s + c0, sr);
+  }
+  tmem_st_wait();
+  move_reference<D>(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), m_ref, l_sum, taddr_o);
+  const float nref = m_ref == -INFINITY ? 0.f : -m_ref;
+  float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int c0 = 0; c0 < 128; c0 += 32) {
+    uint32_t zr[32], pk[16];
+    tmem_ld32(taddr_s + c0, zr);
+    tmem_ld_wait();
+    float* z = reinterpret_cast<float*>(zr);
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      const float4 inv = *reinterpret_cast<const float4*>(scales + 2 * kBN + c0 + i);
+      float p[4];
+      fadd2(p[0], p[1], z[i], z[i + 1], nref, nref);
+      fadd2(p[2], p[3], z[i + 2], z[i + 3], nref, nref);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = ex2(p[e]);
+      ffma2(ps[0], ps[1], p[0], p[1], inv.x, inv.y, ps[0], ps[1]);
+      ffma2(ps[2], ps[3], p[2], p[3], inv.z, inv.w, ps[2], ps[3]);
+      pk[i / 2] = pack2<__half>(p[0], p[1]);
+      pk[i / 2 + 1] = pack2<__half>(p[2], p[3]);
+    }
+    tmem_st16(taddr_s + c0 / 2, pk);
+    if (c0 & 32) publish_half(&bars[c0 / 64]);
+  }
+  l_sum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
 }
 
 // --------------------------------------------------------------------------------------------
@@ -209,8 +321,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
                   const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   using G = Geometry<D, kInt8>;
-  using P = typename std::conditional<kInt8, __half, T>::type;   // weights, and V as multiplied
-  using Sh = Shared<G::kKSlots, G::kVSlots, G::kCodeSlots>;
+  using Sh = Shared<G::kKSlots, G::kVSlots, G::kCodeSlots, G::kScaleSlots>;
   constexpr int kKSlots = G::kKSlots, kVSlots = G::kVSlots;
   constexpr int kTileBytes = G::kTileBytes;
   extern __shared__ uint8_t smem_raw[];
@@ -238,7 +349,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
       mbar_init(&sh->code_full[i], 1);
       mbar_init(&sh->code_empty[i], 128);
     }
-    for (int i = 0; i < kScaleSlots; ++i) mbar_init(&sh->scale_full[i], 128);
+    for (int i = 0; i < G::kScaleSlots; ++i) mbar_init(&sh->scale_full[i], 128);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh->q_full[t], 1);
       mbar_init(&sh->q_free[t], 1);
@@ -376,9 +487,9 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     // ------------------------------- MMA issuer -------------------------------
     // The warp runs this loop together; one lane issues every tcgen05.mma and commit. A one-tile
     // item's second chain reads Q tile 0 as well.
-    constexpr int kFmtQk = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-    constexpr int kFmtPv = std::is_same<P, __nv_bfloat16>::value ? 1 : 0;
-    constexpr uint32_t kIdescQk = umma_idesc_f16(kFmtQk, kBM, kBN, 0);
+    constexpr int kFmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+    constexpr int kFmtPv = kInt8 ? 0 : kFmt;
+    constexpr uint32_t kIdescQk = umma_idesc_f16(kFmt, kBM, kBN, 0);
     constexpr uint32_t kIdescPv = umma_idesc_f16(kFmtPv, kBM, D, 1);
     const bool leader = elect_one();
     const Desc q_desc(umma_smem_desc_sw128(smem_u32(q_smem), 16, 1024));
@@ -497,7 +608,6 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     const uint32_t lane_field = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t taddr_s = tmem + c * 128 + lane_field;
     const uint32_t taddr_o = tmem + 256 + c * 128 + lane_field;
-    const float sl2 = a.scale_log2;
     const int row_token = row / a.group;
     const int row_head = row - row_token * a.group;
     int s_waits = 0, o_waits[2] = {0, 0}, joins = 0;
@@ -534,77 +644,23 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
           continue;
         }
         tc_fence_after();
-        uint32_t sr[128];
-        tmem_ld32(taddr_s + 0, *reinterpret_cast<uint32_t(*)[32]>(&sr[0]));
-        tmem_ld32(taddr_s + 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[32]));
-        tmem_ld32(taddr_s + 64, *reinterpret_cast<uint32_t(*)[32]>(&sr[64]));
-        tmem_ld32(taddr_s + 96, *reinterpret_cast<uint32_t(*)[32]>(&sr[96]));
-        tmem_ld_wait();
-        float* sf = reinterpret_cast<float*>(sr);
         const int k0 = s.tile(c, j) * kBN;
-        const float* scales = nullptr;
+        const bool masked = k0 + kBN > s.seq.len ||
+                            (a.causal && k0 + kBN - 1 > offset + tile_first);
         if constexpr (kInt8) {
-          // z = s mult + add.
           const int at = kv_base + s.place(c, j);
-          if (!mbar_wait(&sh->scale_full[at % kScaleSlots], (at / kScaleSlots) & 1, guard)) {
+          if (!mbar_wait(&sh->scale_full[at % G::kScaleSlots], (at / G::kScaleSlots) & 1, guard)) {
             ok = false;
             break;
           }
-          scales = reinterpret_cast<const float*>(smem + G::kScaleOffset) +
-                   (at % kScaleSlots) * 3 * kBN;
-#pragma unroll
-          for (int i = 0; i < 128; i += 4) {
-            const float4 mul = *reinterpret_cast<const float4*>(scales + i);
-            const float4 add = *reinterpret_cast<const float4*>(scales + kBN + i);
-            ffma2(sf[i], sf[i + 1], sf[i], sf[i + 1], mul.x, mul.y, add.x, add.y);
-            ffma2(sf[i + 2], sf[i + 3], sf[i + 2], sf[i + 3], mul.z, mul.w, add.z, add.w);
-          }
+          const float* scales = reinterpret_cast<const float*>(smem + G::kScaleOffset) +
+                                (at % G::kScaleSlots) * 3 * kBN;
+          softmax_tile_int8<D>(taddr_s, taddr_o, scales, masked, limit - k0, m_ref, l_sum,
+                                  sh->p_half[c]);
+        } else {
+          softmax_tile<T, D>(taddr_s, taddr_o, a.scale_log2, masked, limit - k0, m_ref, l_sum,
+                             sh->p_half[c]);
         }
-        const bool masked = k0 + kBN > s.seq.len ||
-                            (a.causal && k0 + kBN - 1 > offset + tile_first);
-        if (masked) {
-          const int visible = limit - k0;  // keys [k0, k0 + visible) are visible to this row
-#pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            if (i >= visible) sf[i] = -INFINITY;
-          }
-        }
-        float mx8[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mx8[i] = fmaxf(sf[i], sf[i + 8]);
-#pragma unroll
-        for (int i0 = 16; i0 < 128; i0 += 16) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) mx8[i] = fmax3(mx8[i], sf[i0 + 2 * i], sf[i0 + 2 * i + 1]);
-        }
-        const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]),
-                               fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-        const float mt = kInt8 ? mx : (mx == -INFINITY ? -INFINITY : mx * sl2);
-
-        // The reference point moves only when the maximum passes it by more than 2^8.
-        float m_new = m_ref;
-        if (m_ref == -INFINITY || mt > m_ref + kRescaleThreshold) m_new = fmaxf(m_ref, mt);
-        const bool rescale = (m_new != m_ref) && (m_ref != -INFINITY);
-        const float factor = rescale ? ex2(m_ref - m_new) : 1.f;
-        if (rescale) l_sum *= factor;
-        m_ref = m_new;
-        const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-        if (__any_sync(0xffffffffu, rescale)) {
-          // P V of the chain's previous step has completed (s_full covers it) and this step's waits
-          // for the first half of P.
-#pragma unroll 1
-          for (int i = 0; i < D / 16; ++i) {
-            uint32_t ov[16];
-            tmem_ld16(taddr_o + i * 16, ov);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * factor);
-            tmem_st16(taddr_o + i * 16, ov);
-          }
-        }
-        float ps[4] = {0.f, 0.f, 0.f, 0.f};
-        exp_store<P, kInt8>(sf, sl2, -ref, scales + 2 * kBN, ps, taddr_s, sh->p_half[c]);
-        l_sum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
       }
       if (!ok) break;
       kv_base += s.t1 - s.t0;
@@ -717,34 +773,43 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kOtherRegs));
     if constexpr (kInt8) {
       // ------------------------------- code converters -------------------------------
-      // Thread r also holds key r of the tile: its scales are read one tile ahead, its block two.
-      // A tile's scales go to slot (tile % kScaleSlots) before its K tile is published. The slot is
-      // free: the V tile two before this K tile has been converted, so P V of the tile kVSlots
-      // earlier than that one has run, which follows its softmax (and kVSlots + 2 <= kScaleSlots).
-      const int tid = threadIdx.x - kConvertWarp * 32;
+      // One warpgroup for K, one for V. Code tiles arrive in the producer's order: of a segment's n
+      // key tiles K 0, K 1, V 0, K 2, V 1, ..., V n - 1.
+      const bool is_v = warp >= kConvertWarp + 4;
+      const int tid = threadIdx.x - (is_v ? kConvertWarp + 4 : kConvertWarp) * 32;
       const bool paged = a.cache.block_tables != nullptr;
-      static_assert(kVSlots + 2 <= kScaleSlots, "a tile's scales outlive its softmax");
-      int k_done = 0, v_done = 0;   // tiles converted
+      int base = 0;   // key tiles of earlier segments
       bool ok = true;
-      // The next code tile, once it and its place in the 16-bit ring are there.
-      auto ready = [&](bool is_v, const uint8_t*& codes, uint8_t*& dst) -> bool {
-        const int n = k_done + v_done, slot = n % G::kCodeSlots;
-        const int at = is_v ? v_done : k_done, slots = is_v ? kVSlots : kKSlots;
-        uint64_t* empty = is_v ? &sh->v_empty[at % slots] : &sh->k_empty[at % slots];
-        codes = smem + G::kCodeOffset + slot * G::kCodeBytes;
-        dst = (is_v ? v_ring : k_ring) + (at % slots) * kTileBytes;
-        return mbar_wait(&sh->code_full[slot], (n / G::kCodeSlots) & 1, guard) &&
-               (at < slots || mbar_wait(empty, ((at / slots) - 1) & 1, guard));
-      };
-      auto publish = [&](bool is_v) {
+      // Key tile i of the segment, once it and its place in the 16-bit ring are there.
+      auto convert = [&](int i, int n) -> bool {
+        const int code = 2 * base + (is_v ? (i + 1 < n ? 2 * i + 2 : 2 * i + 1) : max(2 * i - 1, 0));
+        const int code_slot = code % G::kCodeSlots;
+        const int at = base + i, slots = is_v ? kVSlots : kKSlots, slot = at % slots;
+        uint64_t* empty = is_v ? &sh->v_empty[slot] : &sh->k_empty[slot];
+        if (!mbar_wait(&sh->code_full[code_slot], (code / G::kCodeSlots) & 1, guard) ||
+            (at >= slots && !mbar_wait(empty, ((at / slots) - 1) & 1, guard)))
+          return false;
+        const uint8_t* codes = smem + G::kCodeOffset + code_slot * G::kCodeBytes;
+        if (is_v) {
+          convert_tile<__half, D>(codes, v_ring + slot * kTileBytes, tid);
+        } else {
+          convert_tile<T, D>(codes, k_ring + slot * kTileBytes, tid);
+        }
         fence_proxy_async_shared();
-        mbar_arrive(is_v ? &sh->v_full[v_done % kVSlots] : &sh->k_full[k_done % kKSlots]);
-        mbar_arrive(&sh->code_empty[(k_done + v_done) % G::kCodeSlots]);
-        ++(is_v ? v_done : k_done);
+        mbar_arrive(is_v ? &sh->v_full[slot] : &sh->k_full[slot]);
+        mbar_arrive(&sh->code_empty[code_slot]);
+        return true;
       };
       walk.start(a, sh->share);
       while (ok && walk.next(a, s)) {
-        if (s.tiles == 0) continue;
+        const int n = s.t1 - s.t0;
+        if (is_v) {
+          for (int i = 0; ok && i < n; ++i) ok = convert(i, n);
+          base += n;
+          continue;
+        }
+        // Thread r of the K warpgroup also holds key r of the tile: its scales are read one tile
+        // ahead, its block two.
         const int32_t* table = a.cache.block_tables + s.b * a.cache.bt_stride;
         auto block_of = [&](int tile) -> int {
           if (!paged) return s.b;
@@ -764,42 +829,42 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
                             s.hkv * a.cache.vs_stride[2]];
           }
         };
-        float sk, sv;
-        scales_of(s.t0, block_of(s.t0), sk, sv);
-        int blk_next = block_of(s.t0 + 1);
-        for (int i = s.t0; ok && i <= s.t1; ++i) {   // K tile i, V tile i - 1
-          const uint8_t* codes;
-          uint8_t* dst;
-          if (i < s.t1) {
-            float sk_next = 0.f, sv_next = 0.f;
-            if (i + 1 < s.t1) {
-              scales_of(i + 1, blk_next, sk_next, sv_next);
-              blk_next = block_of(i + 2);
-            }
-            ok = ready(false, codes, dst);
-            if (!ok) break;
-            // Keys past the length have no weight. A scale that is not finite makes z, and so the
-            // weight, not finite for the rows that see the key, and adds nothing to others' sums.
-            float* out = reinterpret_cast<float*>(smem + G::kScaleOffset) +
-                         (k_done % kScaleSlots) * 3 * kBN + tid;
-            const bool in = i * kBN + tid < s.seq.len;
-            sv = sv < kMinScale ? kMinScale : sv;
-            out[0] = in ? sk * a.scale_log2 : 0.f;
-            out[kBN] = in ? __log2f(sv) : -INFINITY;
-            out[2 * kBN] = in && sv <= 0x1p+127f ? 1.f / sv : 0.f;
-            mbar_arrive(&sh->scale_full[k_done % kScaleSlots]);
-            convert_tile<T, D>(codes, dst, tid);
-            publish(false);
-            sk = sk_next;
-            sv = sv_next;
-          }
-          if (i > s.t0) {
-            ok = ready(true, codes, dst);
-            if (!ok) break;
-            convert_tile<__half, D>(codes, dst, tid);
-            publish(true);
-          }
+        float sk = 0.f, sv = 0.f;
+        int blk_next = 0;
+        if (n > 0) {
+          scales_of(s.t0, block_of(s.t0), sk, sv);
+          blk_next = block_of(s.t0 + 1);
         }
+        for (int i = 0; ok && i < n; ++i) {
+          float sk_next = 0.f, sv_next = 0.f;
+          if (i + 1 < n) {
+            scales_of(s.t0 + i + 1, blk_next, sk_next, sv_next);
+            blk_next = block_of(s.t0 + i + 2);
+          }
+          // The place of these scales is free once K 's is (see kScaleSlots).
+          const int at = base + i;
+          if (at >= kKSlots &&
+              !mbar_wait(&sh->k_empty[at % kKSlots], ((at / kKSlots) - 1) & 1, guard)) {
+            ok = false;
+            break;
+          }
+          float* out = reinterpret_cast<float*>(smem + G::kScaleOffset) +
+                       (at % G::kScaleSlots) * 3 * kBN + tid;
+          // Keys past the length have no weight.
+          const bool in = (s.t0 + i) * kBN + tid < s.seq.len;
+          const bool finite = sv <= 0x1p+127f;
+          // A V scale that is not finite makes the score NaN: it reaches the rows that see the key
+          // and adds nothing to the sums of the others.
+          out[0] = !in ? 0.f : finite ? sk * a.scale_log2 : __int_as_float(0x7fffffff);
+          sv = sv < kMinScale ? kMinScale : sv;
+          out[kBN] = !in ? -INFINITY : finite ? __log2f(sv) : 0.f;
+          out[2 * kBN] = in && finite ? 1.f / sv : 0.f;
+          mbar_arrive(&sh->scale_full[at % G::kScaleSlots]);
+          sk = sk_next;
+          sv = sv_next;
+          ok = convert(i, n);
+        }
+        base += n;
       }
     }
   } else {
@@ -918,7 +983,8 @@ template <typename T, int D, bool kInt8>
 int launch(const ExtendArgs& a, const CUtensorMap& tmq, const CUtensorMap& tmk,
            const CUtensorMap& tmv, int ctas, int dev, cudaStream_t stream) {
   using G = Geometry<D, kInt8>;
-  constexpr int kSmem = G::kTailOffset + static_cast<int>(sizeof(Shared<G::kKSlots, G::kVSlots, G::kCodeSlots>)) +
+  constexpr int kSmem = G::kTailOffset + static_cast<int>(sizeof(Shared<G::kKSlots, G::kVSlots, G::kCodeSlots,
+                                                               G::kScaleSlots>)) +
                         1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
   auto kernel = extend_kernel<T, D, kInt8>;
