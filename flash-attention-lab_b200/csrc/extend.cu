@@ -335,7 +335,8 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
+  // Warp 0 finds the share, which takes longest: the other preparations are other warps'.
+  if (warp == kMmaWarp && lane == 0) {
     sh->abort_flag = 0;
     for (int i = 0; i < kKSlots; ++i) {
       mbar_init(&sh->k_full[i], kInt8 ? 128 : 1);
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
   const uint32_t tmem = sh->tmem_base;
   const WaitGuard guard{reinterpret_cast<volatile int*>(&sh->abort_flag), a.status};
   Walk walk;
-  Segment s;
+  Segment s{};
 
   // Barrier phases run on across segments: each role counts the completions it has waited for.
   if (warp == kProducerWarp) {
@@ -881,16 +882,20 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
   }
 }
 
-// Joins the partials of the items that were cut. Block (c, y) handles the item that CTA c opened
-// without closing, if there is one: its parts are that slot and the first slots of the following
-// CTAs, up to the one that closes it, combined in that order (CTAs whose share held no whole key
-// tile of the item left none). A thread owns 8 columns of one row.
+// Joins the partials of the items that were cut, of one launch or (blocks past the first `ctas`) of
+// two. Block (c, y) handles the item that CTA c opened without closing, if there is one: its parts
+// are that slot and the first slots of the following CTAs, up to the one that closes it, combined
+// in that order (CTAs whose share held no whole key tile of the item left none). A thread owns 8
+// columns of one row.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) extend_merge_kernel(const __grid_constant__ ExtendArgs a,
+__global__ void __launch_bounds__(256) extend_merge_kernel(const __grid_constant__ ExtendArgs first,
+                                                           const __grid_constant__ ExtendArgs second,
                                                            int ctas) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const bool is_first = static_cast<int>(blockIdx.x) < ctas;
+  const ExtendArgs& a = is_first ? first : second;
   __shared__ int first_flags[kMaxCtas];   // flags of the CTAs' first slots
-  const int cta = blockIdx.x;
+  const int cta = is_first ? blockIdx.x : blockIdx.x - ctas;
   int open = -1;
   int4 meta = make_int4(0, 0, 0, 0);
   const int4 m0 = a.part_meta[2 * cta], m1 = a.part_meta[2 * cta + 1];
@@ -1007,25 +1012,27 @@ int launch(const ExtendArgs& a, const CUtensorMap& tmq, const CUtensorMap& tmk,
   return check_cuda(cudaGetLastError(), "extend_kernel launch");
 }
 
+// Merges the partials of `count` (1 or 2) launches.
 template <typename T, int D>
-int launch_merge(const ExtendArgs& a, int ctas, cudaStream_t stream) {
+int launch_merge(const ExtendArgs* a, int count, int ctas, cudaStream_t stream) {
+  const int rows = std::max(a[0].part_rows, a[count - 1].part_rows);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, (a.part_rows * (D / 8) + 255) / 256);
+  cfg.gridDim = dim3(count * ctas, (rows * (D / 8) + 255) / 256);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[1];   // scheduled while the last launch drains
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, extend_merge_kernel<T, D>, a, ctas),
+  return check_cuda(cudaLaunchKernelEx(&cfg, extend_merge_kernel<T, D>, a[0], a[count - 1], ctas),
                     "extend_merge_kernel launch");
 }
 
 template <typename T>
-int launch_merge_t(int head_dim, const ExtendArgs& a, int ctas, cudaStream_t stream) {
-  return head_dim == 128 ? launch_merge<T, 128>(a, ctas, stream)
-                         : launch_merge<T, 64>(a, ctas, stream);
+int launch_merge_t(int head_dim, const ExtendArgs* a, int count, int ctas, cudaStream_t stream) {
+  return head_dim == 128 ? launch_merge<T, 128>(a, count, ctas, stream)
+                         : launch_merge<T, 64>(a, count, ctas, stream);
 }
 
 template <typename T>
@@ -1161,9 +1168,12 @@ extern "C" int flb_extend_fwd(const flb_kv_cache* c, const flb_extend_params* p,
   a.box_rows = box_rows_for(c);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   char* ws = static_cast<char*>(p->workspace);
-  auto merge = [&](const ExtendArgs& args) {
-    return p->dtype == FLB_BF16 ? launch_merge_t<__nv_bfloat16>(c->head_dim, args, sm_count, stream)
-                                : launch_merge_t<__half>(c->head_dim, args, sm_count, stream);
+  ExtendArgs done[2];   // launches whose partials are to be merged
+  int launches = 0;
+  auto merge = [&] {
+    return p->dtype == FLB_BF16
+               ? launch_merge_t<__nv_bfloat16>(c->head_dim, done, launches, sm_count, stream)
+               : launch_merge_t<__half>(c->head_dim, done, launches, sm_count, stream);
   };
 
   // Which kernel: by the rows of every sequence when they are known here, else both (int8).
@@ -1176,14 +1186,16 @@ extern "C" int flb_extend_fwd(const flb_kv_cache* c, const flb_extend_params* p,
     ExtendArgs f = a;
     f.tile_tokens = many ? kFewTile / a.group : static_cast<int>(per_seq);
     f.select = many ? kFewRows : kAllRows;
+    f.item_tokens = FastDiv::of(2 * f.tile_tokens);
     set_partials(&f, ws, sm_count, kFewTile);
     if (int st = launch_extend_few(f, c, p->q, p->q_row_stride, p->q_head_stride, p->dtype,
                                    sm_count, dev, stream))
       return st;
-    if (int st = merge(f)) return st;
+    done[launches++] = f;
   }
-  if (!many) return FLB_OK;
+  if (!many) return merge();
   a.tile_tokens = kBM / a.group;
+  a.item_tokens = FastDiv::of(2 * a.tile_tokens);
   a.select = few ? kManyRows : kAllRows;
   set_partials(&a, ws + partial_bytes(sm_count, kFewTile, c->head_dim), sm_count,
                part_rows(p->rows, a.group));
@@ -1202,5 +1214,7 @@ extern "C" int flb_extend_fwd(const flb_kv_cache* c, const flb_extend_params* p,
   const int st = p->dtype == FLB_BF16
                      ? launch_t<__nv_bfloat16>(c, a, tmq, tmk, tmv, sm_count, dev, stream)
                      : launch_t<__half>(c, a, tmq, tmk, tmv, sm_count, dev, stream);
-  return st != FLB_OK ? st : merge(a);
+  if (st != FLB_OK) return st;
+  done[launches++] = a;
+  return merge();
 }

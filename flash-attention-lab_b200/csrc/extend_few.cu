@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
+  if (warp == G::kScaleWarp && lane == 0) {   // warp 0 finds the share
     sh->abort_flag = 0;
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sh->full[i], 34);   // the bytes of K and of V, and each lane's scales
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
   __syncthreads();
   const WaitGuard guard{reinterpret_cast<volatile int*>(&sh->abort_flag), a.status};
   Walk walk;
-  Segment s;
+  Segment s{};
   walk.start(a, sh->share);
 
   if (warp < G::kScaleWarp && warp >= G::kCopyWarp) {

@@ -32,6 +32,7 @@ struct ExtendArgs {
   int* status;
   int heads, group, causal;
   int tile_tokens;                    // tokens per tile: (128, or 16 in extend_few.cu) / group
+  FastDiv item_tokens;                // 2 tile_tokens
   int select;                         // kAllRows, or which sequences this launch takes
   int wide_scales;                    // extend_few.cu: scales are read 16 bytes at a time
   int box_rows;                       // cache rows per TMA box (a box never crosses a page)
@@ -91,7 +92,7 @@ __device__ __forceinline__ int tiles_seen(const ExtendArgs& a, const Sequence& s
 
 // Item k of a sequence: tokens [k 2 tt, (k + 1) 2 tt). Its cost in units.
 __device__ __forceinline__ int items_of(const ExtendArgs& a, const Sequence& s) {
-  return (s.n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens);
+  return a.item_tokens.div(s.n + a.item_tokens.d - 1);
 }
 __device__ __forceinline__ int item_units(const ExtendArgs& a, const Sequence& s, int k) {
   const int first = k * 2 * a.tile_tokens;
@@ -252,7 +253,7 @@ __device__ __forceinline__ void share_bounds(int64_t total, int64_t& g0, int64_t
 __device__ __forceinline__ void find_share(const ExtendArgs& a, Share* sh, int* pref) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int batch = a.ragged.batch;
-  constexpr int kFew = 4;   // items one thread sums by itself
+  constexpr int kFew = 16;   // items one thread sums by itself
   int64_t g0, g1;
   if (batch <= 32) {
     if (warp != 0) return;
