@@ -148,7 +148,7 @@ struct Walk {
       s.tiles = tiles_seen(a, seq, s.first + s.tokens);
       const int weight = s.dual ? 1 : 2;
       const int total = kItemUnits + weight * s.tiles;
-      const int from = at;
+      const int from = min(at, total);
       const int to = static_cast<int>(min(static_cast<int64_t>(total), at + left));
       s.t0 = (max(from - kItemUnits, 0) + weight - 1) / weight;
       s.t1 = (max(to - kItemUnits, 0) + weight - 1) / weight;
@@ -162,7 +162,10 @@ struct Walk {
             do {   // some later sequence has rows, or the next head's first: units are left
               if (++b >= a.ragged.batch) {
                 b = 0;
-                ++hkv;
+                if (++hkv >= a.cache.heads_kv) {   // offsets that decrease promise too many
+                  left = 0;
+                  break;
+                }
               }
               seq = load_sequence(a, b);
             } while (seq.n == 0);
@@ -231,7 +234,7 @@ __device__ __forceinline__ void locate_unit(const ExtendArgs& a, Share* sh, int 
     sh->b = b;
     sh->hkv = hkv;
     sh->k = k;
-    sh->at = rem - before;
+    sh->at = max(rem - before, 0);
   }
 }
 
@@ -280,7 +283,7 @@ __device__ __forceinline__ void find_share(const ExtendArgs& a, Share* sh, int* 
     if (g1 > g0) {
       const int hkv = static_cast<int>(divide(g0, total));
       const int rem = static_cast<int>(g0 - static_cast<int64_t>(hkv) * total);
-      const int b = __ffs(__ballot_sync(0xffffffffu, incl > rem)) - 1;
+      const int b = max(__ffs(__ballot_sync(0xffffffffu, incl > rem)) - 1, 0);
       locate_unit(a, sh, hkv, b, sequence_of(b), rem - __shfl_sync(0xffffffffu, incl - own, b),
                   lane);
     }

@@ -371,6 +371,8 @@ int validate_kv_cache(const flb_kv_cache* c) {
   if (c->batch <= 0 || c->heads_kv <= 0 || c->max_seqlen <= 0)
     return fail(FLB_ERR_INVALID_ARGUMENT, "empty cache: batch %d heads_kv %d S_max %d", c->batch,
                 c->heads_kv, c->max_seqlen);
+  if (c->max_seqlen > kMaxSeqlen)
+    return fail(FLB_ERR_UNSUPPORTED, "S_max %d is more than %d", c->max_seqlen, kMaxSeqlen);
   if (c->dtype != FLB_BF16 && c->dtype != FLB_FP16 && c->dtype != FLB_FP32 &&
       c->dtype != FLB_INT8)
     return fail(FLB_ERR_UNSUPPORTED, "a cache is bf16, fp16, fp32 or int8 (dtype code %d)",

@@ -26,6 +26,9 @@ struct FastDiv {
   }
 };
 
+// Keys per sequence: positions of the tile behind the last key stay in 31 bits.
+constexpr int kMaxSeqlen = 1 << 30;
+
 // A KV cache as the kernels see it. Strides in elements of the cache (or of the scales).
 struct KvView {
   void* k;

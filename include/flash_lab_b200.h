@@ -319,6 +319,9 @@ typedef struct {
   int32_t dtype;         /* FLB_BF16, FLB_FP16 or FLB_FP32 */
 } flb_kv_rows;
 
+/* cu_seqlens must not decrease: where it does, rows are written by several sequences or by none, but
+ * nothing outside the buffers is touched. max_seqlen is at most 2^30. */
+
 /* Writes each sequence's rows into the cache at its last positions: with n rows, row i of sequence
  * b becomes key seq_lens[b] - n + i. Rows that belong to no sequence, positions outside
  * [0, max_seqlen) and block ids outside [0, num_blocks) are skipped. An FLB_INT8 cache is quantised
@@ -336,7 +339,7 @@ int flb_kv_gather(const flb_kv_cache* cache, const flb_kv_rows* rows, flb_stream
  * flb_kv_rows; lse is [rows, H] fp32. Sequence b has L = seq_lens[b] keys (clamped to
  * [0, max_seqlen]) and its n rows are its last n tokens: row i sees keys 0 .. L - n + i when
  * causal is 1, all L keys otherwise. Rows that see no key or belong to no sequence give 0 and
- * an LSE of -inf. head_dim 64 or 128, H / H_kv at most 128, pages of 8, 16, 32 or a multiple of
+ * an LSE of -inf. head_dim 64 or 128, H / H_kv and sequences at most 128 and 16384, pages of 8, 16, 32 or a multiple of
  * 64 rows; pointers and strides of q, o and the caches are multiples of 16 bytes.
  * workspace holds flb_extend_workspace_bytes(...) bytes; nothing in it needs initialising.
  */

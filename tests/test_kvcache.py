@@ -233,6 +233,61 @@ def test_extend_many_sequences(int8):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("int8", [False, True], ids=["16bit", "int8"])
+@pytest.mark.parametrize("sequences", [3, 40])
+def test_extend_many_items_per_sequence(sequences, int8):
+    # 64 query heads per KV head: an item is four tokens, so a sequence has dozens of them.
+    new = [200 if i % 13 == 1 else i % 3 for i in range(sequences)]
+    cache = Cache([n + 60 for n in new], 2, 64, torch.float16, int8)
+    check_extend(cache, new, 128, torch.float16)
+
+
+@pytest.mark.gpu
+def test_decreasing_offsets_stay_inside_the_buffers():
+    # Not a valid call: its rows are unspecified, but it ends and touches nothing else.
+    cache = Cache([300, 200, 100], 2, 64, torch.bfloat16, page=16)
+    q = torch.randn(64, 8, 64, device="cuda").bfloat16()
+    big = torch.full((64 + 8, 8, 64), -7.0, device="cuda", dtype=torch.bfloat16)
+    for cu in ([0, 64, 0, 64], [64, 0, 64, 0], [10 ** 9, -5, 10 ** 9, 3], [5, 5, 5, 5]):
+        cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
+        out = flash_lab.extend(q, cache.k, cache.v, cache.seq_lens, cu, **cache.kwargs())
+        big[4:-4] = out
+        flash_lab.gather_kv(cache.k, cache.v, cache.seq_lens, cu, 70, **cache.kwargs())
+        torch.cuda.synchronize()
+        assert ops.device_status(0) == 0
+    for b in range(3):   # the cache is as it was
+        k, _ = cache.keys(b)
+        got, _ = flash_lab.gather_kv(cache.k, cache.v, cache.seq_lens, offsets(cache.lens), 600,
+                                     **cache.kwargs())
+        first = sum(cache.lens[:b])
+        assert np.array_equal(host64(got[first:first + len(k)]), k)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    # Pages at the far end of pools of more than 2^31 rows' values: the same bits as in a small pool.
+    page, heads_kv, d, lens = 64, 8, 128, [200, 130]
+    blocks = (1 << 31) // (page * heads_kv * d) + 9
+    k, v = (torch.randn(sum(lens), heads_kv, d, device="cuda").half() for _ in range(2))
+    q = torch.randn(6, 16, d, device="cuda").half()
+    seq_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    results = []
+    for n in (8, blocks):
+        pool = [torch.empty(n, page, heads_kv, d, dtype=torch.int8, device="cuda") for _ in range(2)]
+        scales = dict(k_scale=torch.empty(n, heads_kv, page, device="cuda").transpose(1, 2),
+                      v_scale=torch.empty(n, heads_kv, page, device="cuda").transpose(1, 2))
+        tables = torch.tensor([[n - 1, n - 3, n - 5, n - 7], [n - 2, n - 4, n - 6, 0]],
+                              dtype=torch.int32, device="cuda")
+        flash_lab.append_kv(k, v, *pool, seq_lens, offsets(lens), tables, **scales)
+        results.append((*flash_lab.gather_kv(*pool, seq_lens, offsets(lens), sum(lens), tables,
+                                             dtype=torch.float16, **scales),
+                        flash_lab.extend(q, *pool, seq_lens, offsets([5, 1]), tables, **scales),
+                        flash_lab.extend(q, *pool, seq_lens, offsets([1, 5]), tables, **scales),
+                        flash_lab.decode(q[:2], *pool, seq_lens, tables, **scales)))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True], ids=["16bit", "int8"])
 def test_extend_long_context(int8):
     # One sequence's keys cut over every CTA and merged.
     cache = Cache([9001], 2, 128, torch.bfloat16, int8, page=64)
@@ -833,6 +888,7 @@ def _host_cache(**changes):
 @pytest.mark.parametrize("changes,status,message", [
     (dict(k_cache=0), _capi.FLB_ERR_INVALID_ARGUMENT, b"NULL"),
     (dict(batch=0), _capi.FLB_ERR_INVALID_ARGUMENT, b"empty cache"),
+    (dict(max_seqlen=(1 << 30) + 1), _capi.FLB_ERR_UNSUPPORTED, b"S_max"),
     (dict(dtype=9), _capi.FLB_ERR_UNSUPPORTED, b"dtype code 9"),
     (dict(head_dim=96), _capi.FLB_ERR_UNSUPPORTED, b"head_dim 96"),
     (dict(dtype=_capi.FLB_INT8), _capi.FLB_ERR_INVALID_ARGUMENT, b"needs k_scale"),
