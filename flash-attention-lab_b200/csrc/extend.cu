@@ -887,10 +887,11 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
 // are that slot and the first slots of the following CTAs, up to the one that closes it, combined
 // in that order (CTAs whose share held no whole key tile of the item left none). A thread owns 8
 // columns of one row.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) extend_merge_kernel(const __grid_constant__ ExtendArgs first,
-                                                           const __grid_constant__ ExtendArgs second,
-                                                           int ctas) {
+// kBatch parts' loads are issued together: 8 for launches of few rows, whose items are cut into many
+// parts, 4 (four blocks per SM) for large partials, where most blocks only find nothing to do.
+template <typename T, int D, int kBatch>
+__global__ void __launch_bounds__(256, kBatch == 4 ? 4 : 2) extend_merge_kernel(
+    const __grid_constant__ ExtendArgs first, const __grid_constant__ ExtendArgs second, int ctas) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const bool is_first = static_cast<int>(blockIdx.x) < ctas;
   const ExtendArgs& a = is_first ? first : second;
@@ -898,8 +899,8 @@ __global__ void __launch_bounds__(256) extend_merge_kernel(const __grid_constant
   const int cta = is_first ? blockIdx.x : blockIdx.x - ctas;
   int open = -1;
   int4 meta = make_int4(0, 0, 0, 0);
+  if (static_cast<int>(blockIdx.y) * 256 >= a.part_rows * (D / 8)) return;
   const int4 m0 = a.part_meta[2 * cta], m1 = a.part_meta[2 * cta + 1];
-  for (int i = cta + 1 + threadIdx.x; i < ctas; i += 256) first_flags[i] = a.part_meta[2 * i].x;
   constexpr int kWhich = kPartValid | kPartOpens | kPartCloses;
   if ((m0.x & kWhich) == (kPartValid | kPartOpens)) {
     open = 2 * cta;
@@ -909,6 +910,7 @@ __global__ void __launch_bounds__(256) extend_merge_kernel(const __grid_constant
     meta = m1;
   }
   if (open < 0) return;
+  for (int i = cta + 1 + threadIdx.x; i < ctas; i += 256) first_flags[i] = a.part_meta[2 * i].x;
   __syncthreads();
   const int idx = blockIdx.y * 256 + threadIdx.x;
   const int row = idx % a.part_rows, col = idx / a.part_rows;
@@ -932,7 +934,6 @@ __global__ void __launch_bounds__(256) extend_merge_kernel(const __grid_constant
     }
     return -1;
   };
-  constexpr int kBatch = 8;   // parts whose loads are issued together
   while (slot >= 0) {
     float2 ml[kBatch];
     float4 o0[kBatch], o1[kBatch];
@@ -1012,6 +1013,8 @@ int launch(const ExtendArgs& a, const CUtensorMap& tmq, const CUtensorMap& tmk,
   return check_cuda(cudaGetLastError(), "extend_kernel launch");
 }
 
+constexpr int kFewPartRows = 64;   // rows of a partial up to which a merge has few blocks
+
 // Merges the partials of `count` (1 or 2) launches.
 template <typename T, int D>
 int launch_merge(const ExtendArgs* a, int count, int ctas, cudaStream_t stream) {
@@ -1025,7 +1028,8 @@ int launch_merge(const ExtendArgs* a, int count, int ctas, cudaStream_t stream) 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, extend_merge_kernel<T, D>, a[0], a[count - 1], ctas),
+  auto kernel = rows <= kFewPartRows ? extend_merge_kernel<T, D, 8> : extend_merge_kernel<T, D, 4>;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a[0], a[count - 1], ctas),
                     "extend_merge_kernel launch");
 }
 
@@ -1184,7 +1188,12 @@ extern "C" int flb_extend_fwd(const flb_kv_cache* c, const flb_extend_params* p,
   const bool many = !few || !known;
   if (few) {
     ExtendArgs f = a;
-    f.tile_tokens = many ? kFewTile / a.group : static_cast<int>(per_seq);
+    // With unknown row counts, up to 8 score rows per sequence where the group allows it: the form
+    // of single tokens, which is the faster one by a third.
+    f.tile_tokens = !many                  ? static_cast<int>(per_seq)
+                    : a.group <= kFewTile / 2 ? kFewTile / 2 / a.group
+                                              : 1;
+    f.few_tokens = a.few_tokens = f.tile_tokens;
     f.select = many ? kFewRows : kAllRows;
     f.item_tokens = FastDiv::of(2 * f.tile_tokens);
     set_partials(&f, ws, sm_count, kFewTile);

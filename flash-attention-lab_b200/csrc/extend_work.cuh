@@ -33,7 +33,8 @@ struct ExtendArgs {
   int heads, group, causal;
   int tile_tokens;                    // tokens per tile: (128, or 16 in extend_few.cu) / group
   FastDiv item_tokens;                // 2 tile_tokens
-  int select;                         // kAllRows, or which sequences this launch takes
+  int select;                         // kAllRows, or which sequences this launch takes:
+  int few_tokens;                     // those of at most so many rows, or the others
   int wide_scales;                    // extend_few.cu: scales are read 16 bytes at a time
   int box_rows;                       // cache rows per TMA box (a box never crosses a page)
   float scale_log2;
@@ -48,9 +49,9 @@ struct ExtendArgs {
 };
 
 // A call over an int8 cache whose row counts are only known on the device runs both kernels: the one
-// of extend_few.cu takes the sequences whose rows fit in its tile, the other one the rest.
+// of extend_few.cu takes the sequences of at most few_tokens rows, the other one the rest.
 enum : int { kAllRows = 0, kFewRows = 1, kManyRows = 2 };
-constexpr int kFewTile = 16;          // score rows of a tile in extend_few.cu
+constexpr int kFewTile = 16;          // most score rows of a sequence in extend_few.cu
 
 enum : int { kPartValid = 1, kPartOpens = 2, kPartCloses = 4 };
 
@@ -79,7 +80,7 @@ __device__ __forceinline__ Sequence load_sequence(const ExtendArgs& a, int b) {
     end = s.row0 + min(r.rows_per_seq, r.rows - s.row0);
   }
   s.n = end - s.row0;
-  if (a.select != kAllRows && (s.n <= kFewTile / a.group) != (a.select == kFewRows)) s.n = 0;
+  if (a.select != kAllRows && (s.n <= a.few_tokens) != (a.select == kFewRows)) s.n = 0;
   s.len = min(max(__ldg(a.seq_lens + b), 0), a.cache.max_seqlen);
   return s;
 }

@@ -339,8 +339,9 @@ int flb_kv_gather(const flb_kv_cache* cache, const flb_kv_rows* rows, flb_stream
  * flb_kv_rows; lse is [rows, H] fp32. Sequence b has L = seq_lens[b] keys (clamped to
  * [0, max_seqlen]) and its n rows are its last n tokens: row i sees keys 0 .. L - n + i when
  * causal is 1, all L keys otherwise. Rows that see no key or belong to no sequence give 0 and
- * an LSE of -inf. head_dim 64 or 128, H / H_kv and sequences at most 128 and 16384, pages of 8, 16, 32 or a multiple of
- * 64 rows; pointers and strides of q, o and the caches are multiples of 16 bytes.
+ * an LSE of -inf. head_dim 64 or 128, H / H_kv at most 128, at most 16384 sequences, pages of 8, 16,
+ * 32 or a multiple of 64 rows; pointers and strides of q, o and the caches are multiples of 16
+ * bytes.
  * workspace holds flb_extend_workspace_bytes(...) bytes; nothing in it needs initialising.
  */
 typedef struct {
