@@ -28,8 +28,8 @@
 //    a long cache with few rows spreads over all SMs and ragged batches stay balanced. Every CTA
 //    finds its share from cu_seqlens and seq_lens on the device. An item that is cut leaves fp32
 //    partials (at most two per CTA) that extend_merge_kernel joins in key order.
-//  * Warps: two softmax warpgroups, a TMA producer, the MMA issuer, and for int8 a warpgroup that
-//    turns [128 x D] code tiles into the 16-bit tiles the tensor cores read.
+//  * Warps: two softmax warpgroups, a TMA producer, the MMA issuer, and for int8 a warpgroup each for
+//    K and V that turns [128 x D] code tiles into the 16-bit tiles the tensor cores read.
 //  * Keys past a sequence's length are masked in S and their V rows are zeroed in shared memory
 //    (cache rows past the length may hold anything, and 0 * NaN is NaN).
 #include <cuda.h>
@@ -81,7 +81,7 @@ struct Geometry {
   // The register split (setmaxnreg) must not exceed what the CTA is launched with.
   static constexpr int kLaunchRegs = kInt8 ? 96 : 168;
   static constexpr int kSoftmaxRegs = kInt8 ? 128 : 216;
-  static constexpr int kOtherRegs = kInt8 ? 72 : 72;
+  static constexpr int kOtherRegs = 72;
   static_assert(2 * 128 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs <= kThreads * kLaunchRegs,
                 "the register split must fit in the launch's registers");
   static_assert(kMaxBatch * 4 <= kSlots * kTileBytes, "prefix sums fit in the rings");
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
           const float* scales = reinterpret_cast<const float*>(smem + G::kScaleOffset) +
                                 (at % G::kScaleSlots) * 3 * kBN;
           softmax_tile_int8<D>(taddr_s, taddr_o, scales, masked, limit - k0, m_ref, l_sum,
-                                  sh->p_half[c]);
+                               sh->p_half[c]);
         } else {
           softmax_tile<T, D>(taddr_s, taddr_o, a.scale_log2, masked, limit - k0, m_ref, l_sum,
                              sh->p_half[c]);

@@ -1,20 +1,19 @@
 // Attention of a few new rows per sequence over an int8 KV cache: single-token decode, and chunks
 // whose (tokens x query heads of one KV head) are at most 16 score rows. Same operator, work split
 // and partials as extend.cu; HBM bound (2 H_kv (D + 4) bytes per key), so the codes go from shared
-// memory straight into the registers of 16 x 8 x 16 warp MMAs instead of through 16-bit tiles (the
-// tcgen05 form of extend.cu took 297 us for 8 sequences of 24K keys, H_kv 8, D 128).
+// memory straight into the registers of 16 x 8 x 16 warp MMAs instead of through 16-bit tiles. One
+// row of 8 sequences of 24K keys, 32 query and 8 KV heads, D 128 (415 MB): 80 us with the merge,
+// 5.2 TB/s; the first tcgen05 form of extend.cu took 297 us.
 //
 //  * One CTA per SM: two warps stream [128 keys x D] tiles of K and of V codes by TMA, one turns the
-//    keys' scales into what the scores need (below) beside them in the ring stage, and consumer
-//    warps take 16 keys of a tile each (two groups of eight warps on alternate tiles, or one),
-//    every warp with its own online softmax; their results are joined in a fixed order at the
-//    end of a segment. Block tables are read 32 entries at a time. (One producer warp for copies and scales, with a table load per key, bounded 16-row
-//    pages: 5000 clocks per tile where the consumers took 2400.)
+//    keys' scales into what the scores need (below) beside them in the ring stage, and eight consumer
+//    warps take 16 keys of a tile each, every warp with its own online softmax; their results are
+//    joined in a fixed order at the end of a segment. (One producer warp for copies and scales, with
+//    a table load per key, bounded 16-row pages: 5000 clocks per tile where the consumers took 2400.
+//    Sixteen consumers in two groups on alternate tiles: 137 us against 129 with eight, whose issue
+//    slots are 43 % used.)
 //  * Keys are the M rows of the MMAs and score rows their N columns, in one or two blocks of 8: the
-//    usual group of up to 8 heads costs half the MMAs, exponentials and registers of 16 score rows,
-//    and the registers buy the second group of consumers, without which latency bound the
-//    kernel (2.5 warps per scheduler, 40 % of the issue slots, 1900 clocks per tile against the
-//    1400 that HBM needs).
+//    usual group of up to 8 heads costs half the MMAs, exponentials and registers of 16 score rows.
 //  * Q is the B operand, in fp16: bf16 queries are scaled to [1, 2) of their row's maximum by a
 //    power of two, which is exact down to 2^-17 of the maximum and off by at most 2^-25 of it
 //    below. The order of a dot product is free, so thread t of a quad takes D / 4 consecutive values
@@ -31,15 +30,12 @@
 namespace flb {
 namespace {
 
-constexpr int kGroupWarps = 8;        // consumers of one tile: 16 keys each
-static_assert(kGroupWarps * 16 == kBN, "a group covers a tile");
+constexpr int kWarps = kBN / 16;      // consumers: 16 keys of a tile each
 
 // kBlocks: 8-row blocks of score rows (1 or 2).
 template <int D, int kBlocks>
 struct FewGeometry {
   static constexpr int kRows = 8 * kBlocks;
-  static constexpr int kGroups = 1;   // consumer groups, on alternate tiles
-  static constexpr int kWarps = kGroups * kGroupWarps;
   static constexpr int kCopyWarp = kWarps;               // TMA of K, and kCopyWarp + 1 of V
   static constexpr int kScaleWarp = kWarps + 2;
   static constexpr int kThreads = (kWarps + 3) * 32;
@@ -169,7 +165,6 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   using G = FewGeometry<D, kBlocks>;
   constexpr int kStages = G::kStages;
-  constexpr int kWarps = G::kWarps;
   constexpr int kRows = G::kRows;
   constexpr int kSteps = D / 16;    // MMA steps over head_dim, and 16-column chunks of V
   extern __shared__ uint8_t smem_raw[];
@@ -183,7 +178,7 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
     sh->abort_flag = 0;
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sh->full[i], 34);   // the bytes of K and of V, and each lane's scales
-      mbar_init(&sh->empty[i], kGroupWarps);
+      mbar_init(&sh->empty[i], kWarps);
     }
     fence_barrier_init();
   }
@@ -333,12 +328,11 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
   // ------------------------------- consumers -------------------------------
   const int g = lane >> 2;    // fragment row group
   const int t4 = lane & 3;    // thread in quad
-  const int group = warp / kGroupWarps, slice = warp % kGroupWarps;   // tiles, and keys in a tile
   float* join_m = reinterpret_cast<float*>(smem + G::kJoinOffset);   // [warps][kRows]
   float* join_l = join_m + kWarps * kRows;
   float* join_o = join_l + kWarps * kRows;                           // [warps][kRows][D]
   const uint32_t smem_base = smem_u32(smem);
-  const uint32_t v_row = static_cast<uint32_t>(slice * 16 + ((lane >> 3) & 1) * 8 + (lane & 7));
+  const uint32_t v_row = static_cast<uint32_t>(warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7));
   const uint32_t v_chunk = static_cast<uint32_t>(lane >> 4);
   int base = 0;               // tiles of earlier segments
   int segments = 0;
@@ -412,17 +406,15 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
       l_sum[nb][0] = l_sum[nb][1] = 0.f;
     }
 
-    // This group's tiles of the segment: those at ring positions of its parity.
-    const int skip = (group + G::kGroups - base % G::kGroups) % G::kGroups;
-    for (int tile = s.t0 + skip; tile < s.t1; tile += G::kGroups) {
+    for (int tile = s.t0; tile < s.t1; ++tile) {
       const int pos = base + tile - s.t0, st = pos % kStages;
       ok = mbar_wait(&sh->full[st], (pos / kStages) & 1, guard);
       if (!ok) break;
       const uint8_t* kt = smem + 2 * st * G::kTileBytes;
       const uint32_t vt = smem_base + (2 * st + 1) * G::kTileBytes;
       const float* scales = reinterpret_cast<const float*>(smem + G::kScaleOffset +
-                                                           st * G::kScaleBytes) + slice * 16 + g;
-      const int key = tile * kBN + slice * 16 + g;   // and key + 8
+                                                           st * G::kScaleBytes) + warp * 16 + g;
+      const int key = tile * kBN + warp * 16 + g;   // and key + 8
 
       // Two accumulators per block: a chain of D / 16 dependent MMAs is half as long.
       float z[kBlocks][4], y[kBlocks][4];
@@ -438,7 +430,7 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < D / 64; ++i)
             x[r][i] = *reinterpret_cast<const uint4*>(
-                kt + code_offset<D>(slice * 16 + 8 * r + g, t4 * (D / 64) + i));
+                kt + code_offset<D>(warp * 16 + 8 * r + g, t4 * (D / 64) + i));
         }
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {

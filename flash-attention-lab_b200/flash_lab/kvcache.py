@@ -5,8 +5,9 @@ reference, whose decode reads a cache that something else has filled.
 A cache is [B, S_max, H_kv, D], or paged [num_blocks, page_size, H_kv, D] with block_tables
 [B, max_blocks] int32, of the tokens' dtype or int8. An int8 cache holds one fp32 scale per token
 and KV head in k_scale / v_scale, [B, S_max, H_kv] or [num_blocks, page_size, H_kv] with any
-strides: the row x of one token and head is stored as round(x * 127 / max|x|) and max|x| / 127. The
-attention kernels read scales along the keys of one head, so scales stored head by head
+strides: the row x of one token and head is stored as round(x * 127 / max|x|) and max|x| / 127
+(2^-100 at least; the attention kernels read a smaller or negative v_scale as that). The attention
+kernels read scales along the keys of one head, so scales stored head by head
 (`torch.empty(blocks, H_kv, page_size).transpose(1, 2)`) are read with wider loads.
 
 New rows are ragged: [T, H, D] with cu_seqlens [B + 1] int32, where sequence b owns rows
@@ -267,8 +268,8 @@ def extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seq_le
 
     Returns o in q's shape and dtype and, with return_lse=True, the natural-log log-sum-exp of
     each score row as fp32 in q's shape without its last dimension. Rows that see no key, or
-    belong to no sequence, give zeros and -inf. A non-finite value in V makes the whole tile of
-    up to 128 keys around it non-finite for every row that reads the tile, also for rows that the
+    belong to no sequence, give zeros and -inf. One call takes at most 16384 sequences and 128
+    query heads per KV head. A non-finite value in V makes the whole tile of up to 128 keys around it non-finite for every row that reads the tile, also for rows that the
     causal mask keeps from that key (int8 caches: only for the rows that see it); keys at or past
     seq_lens[b] are never read into a result.
     """
