@@ -49,7 +49,7 @@ namespace {
 
 constexpr int kBM = 128;              // score rows per tile
 constexpr int kBoxBytes = kBM * 128;  // a swizzled [128 rows x 64 columns] 16-bit box
-constexpr uint32_t kTmemCols = 512;   // S0 | S1 | O0 | O1
+constexpr uint32_t kTmemCols = 512;   // the S buffers | O0 | O1
 
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
@@ -63,6 +63,10 @@ template <int D, bool kInt8>
 struct Geometry {
   static_assert(D == 64 || D == 128, "head_dim 64 or 128");
   static constexpr int kBoxes = D / 64;
+  // S buffers of 128 TMEM columns that the steps of both chains take in turn: what O leaves.
+  static constexpr int kSBufs = D == 64 ? 3 : 2;
+  static constexpr uint32_t kOCol = kSBufs * 128;        // O of chain 0; chain 1's follows
+  static_assert(kOCol + 2 * D <= kTmemCols, "S and O fit in TMEM");
   static constexpr int kTileBytes = kBM * D * 2;
   static constexpr int kCodeBytes = kBN * D;
   static constexpr int kKSlots = 2 * (128 / D);
@@ -70,8 +74,8 @@ struct Geometry {
   static constexpr int kSlots = kKSlots + kVSlots;
   static constexpr int kCodeSlots = kInt8 ? 3 * (128 / D) : 0;
   // Key tiles whose scales are held: a K tile is converted once Q K^T of the tile kKSlots earlier
-  // has been issued, which follows the softmax of tiles two or more before that one.
-  static constexpr int kScaleSlots = kInt8 ? kKSlots + 2 : 0;
+  // has been issued, which follows the softmax of tiles kSBufs or more before that one.
+  static constexpr int kScaleSlots = kInt8 ? kKSlots + kSBufs : 0;
   static constexpr int kScaleBytes = kScaleSlots * 3 * kBN * 4;
   static constexpr int kRingOffset = 2 * kTileBytes;
   static constexpr int kCodeOffset = kRingOffset + kSlots * kTileBytes;
@@ -87,7 +91,7 @@ struct Geometry {
   static_assert(kMaxBatch * 4 <= kSlots * kTileBytes, "prefix sums fit in the rings");
 };
 
-template <int kKSlots, int kVSlots, int kCodeSlots, int kScaleSlots>
+template <int kKSlots, int kVSlots, int kCodeSlots, int kScaleSlots, int kSBufs>
 struct Shared {
   uint64_t q_full[2];
   uint64_t q_free[2];        // the last Q K^T of an item that reads a Q tile has completed
@@ -98,8 +102,8 @@ struct Shared {
   uint64_t code_full[kCodeSlots + 1];
   uint64_t code_empty[kCodeSlots + 1];
   uint64_t scale_full[kScaleSlots + 1];
-  uint64_t s_full[2];
-  uint64_t p_half[2][2];     // P of keys 0-63 / 64-127 of a tile stored in TMEM
+  uint64_t s_full[kSBufs];
+  uint64_t p_half[kSBufs][2];   // P of keys 0-63 / 64-127 of a tile stored in TMEM
   uint64_t o_full[2];
   uint64_t x_ready, x_done;  // joining the two chains of a one-tile item
   uint64_t mma_done;
@@ -127,6 +131,19 @@ struct Desc {
 };
 constexpr uint32_t kmajor_step(int kk) { return (kk >> 2) * kBoxBytes + (kk & 3) * 32; }
 constexpr uint32_t mnmajor_step(int kk) { return kk * 2048; }
+
+// Whether the phase with the given parity has completed, without waiting.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 
 // --------------------------------------------------------------------------------------------
 // 8-bit codes
@@ -166,12 +183,20 @@ __device__ __forceinline__ void convert_tile(const uint8_t* codes, uint8_t* tile
 // Softmax
 // --------------------------------------------------------------------------------------------
 
+// The barrier phase by which P V of a chain's previous step has completed: the release of its V tile
+// (in a two-tile item by chain 1's P V, which does not wait for this step of either chain).
+struct PrevPv {
+  uint64_t* bar;
+  uint32_t parity;
+};
+
 // The reference point of a row moves only when its maximum mt (log2 domain) passes it by more than
-// 2^8; the row sum and O (in TMEM) follow. P V of the chain's previous step has completed (the
-// scores depend on it) and this step's waits for the first half of P.
+// 2^8; the row sum and O (in TMEM) follow, once P V of the chain's previous step has completed.
+// This step's waits for the first half of P.
 template <int D>
 __device__ __forceinline__ void move_reference(float mt, float& m_ref, float& l_sum,
-                                               uint32_t taddr_o) {
+                                               uint32_t taddr_o, const PrevPv& prev,
+                                               const WaitGuard& guard) {
   float m_new = m_ref;
   if (m_ref == -INFINITY || mt > m_ref + kRescaleThreshold) m_new = fmaxf(m_ref, mt);
   const bool rescale = (m_new != m_ref) && (m_ref != -INFINITY);
@@ -179,6 +204,8 @@ __device__ __forceinline__ void move_reference(float mt, float& m_ref, float& l_
   if (rescale) l_sum *= factor;
   m_ref = m_new;
   if (__any_sync(0xffffffffu, rescale)) {
+    if (!mbar_wait(prev.bar, prev.parity, guard)) return;   // the next wait gives up as well
+    tc_fence_after();
 #pragma unroll 1
     for (int i = 0; i < D / 16; ++i) {
       uint32_t ov[16];
@@ -203,7 +230,8 @@ __device__ __forceinline__ void publish_half(uint64_t* bar) {
 template <typename T, int D>
 __device__ __forceinline__ void softmax_tile(uint32_t taddr_s, uint32_t taddr_o, float sl2,
                                              bool masked, int visible, float& m_ref, float& l_sum,
-                                             uint64_t* bars) {
+                                             uint64_t* bars, const PrevPv& prev,
+                                             const WaitGuard& guard) {
   uint32_t sr[128];
 #pragma unroll
   for (int i = 0; i < 128; i += 32)
@@ -226,7 +254,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t taddr_s, uint32_t taddr_o,
   }
   const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]),
                          fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-  move_reference<D>(mx == -INFINITY ? -INFINITY : mx * sl2, m_ref, l_sum, taddr_o);
+  move_reference<D>(mx == -INFINITY ? -INFINITY : mx * sl2, m_ref, l_sum, taddr_o, prev,
+                    guard);
   const float nref = m_ref == -INFINITY ? 0.f : -m_ref;
   float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -254,7 +283,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t taddr_s, uint32_t taddr_o,
 template <int D>
 __device__ __forceinline__ void softmax_tile_int8(uint32_t taddr_s, uint32_t taddr_o,
                                                   const float* scales, bool masked, int visible,
-                                                  float& m_ref, float& l_sum, uint64_t* bars) {
+                                                  float& m_ref, float& l_sum, uint64_t* bars,
+                                                  const PrevPv& prev, const WaitGuard& guard) {
   float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
   for (int c0 = 0; c0 < 128; c0 += 32) {
@@ -283,7 +313,8 @@ __device__ __forceinline__ void softmax_tile_int8(uint32_t taddr_s, uint32_t tad
     tmem_st32(taddr_s + c0, sr);
   }
   tmem_st_wait();
-  move_reference<D>(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), m_ref, l_sum, taddr_o);
+  move_reference<D>(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), m_ref, l_sum, taddr_o, prev,
+                    guard);
   const float nref = m_ref == -INFINITY ? 0.f : -m_ref;
   float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
@@ -321,7 +352,8 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
                   const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   using G = Geometry<D, kInt8>;
-  using Sh = Shared<G::kKSlots, G::kVSlots, G::kCodeSlots, G::kScaleSlots>;
+  using Sh = Shared<G::kKSlots, G::kVSlots, G::kCodeSlots, G::kScaleSlots, G::kSBufs>;
+  constexpr int kSBufs = G::kSBufs;
   constexpr int kKSlots = G::kKSlots, kVSlots = G::kVSlots;
   constexpr int kTileBytes = G::kTileBytes;
   extern __shared__ uint8_t smem_raw[];
@@ -354,10 +386,12 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh->q_full[t], 1);
       mbar_init(&sh->q_free[t], 1);
-      mbar_init(&sh->s_full[t], 1);
-      mbar_init(&sh->p_half[t][0], kBM);
-      mbar_init(&sh->p_half[t][1], kBM);
       mbar_init(&sh->o_full[t], 1);
+    }
+    for (int i = 0; i < kSBufs; ++i) {
+      mbar_init(&sh->s_full[i], 1);
+      mbar_init(&sh->p_half[i][0], kBM);
+      mbar_init(&sh->p_half[i][1], kBM);
     }
     mbar_init(&sh->x_ready, kBM);
     mbar_init(&sh->x_done, kBM);
@@ -445,7 +479,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
         return blk >= 0 && blk < a.cache.num_blocks ? blk : -1;   // -1 reads as zeros
       };
       auto load_q = [&](int t) -> bool {
-        if (s.dual ? t == 1 : s.count[t] == 0) return true;
+        if (s.dual ? t == 1 : s.count(t) == 0) return true;
         if (q_loads[t] > 0 && !mbar_wait(&sh->q_free[t], (q_loads[t] - 1) & 1, guard)) return false;
         if (lane == 0) {
           mbar_arrive_expect_tx(&sh->q_full[t], q_bytes);
@@ -486,8 +520,12 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
   } else if (warp == kMmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kOtherRegs));
     // ------------------------------- MMA issuer -------------------------------
-    // The warp runs this loop together; one lane issues every tcgen05.mma and commit. A one-tile
-    // item's second chain reads Q tile 0 as well.
+    // One lane waits and issues; the others follow the segments, to help where V rows are zeroed. This
+    // lane's own time bounds the kernel once S has a buffer to spare, so a step's places come from few
+    // operations and P V and the Q K^T behind it are issued in one go. (All lanes waiting together,
+    // with votes, and each step's chain and places from the general formulas: 1450 clocks per step at
+    // head_dim 64, whose MMAs take 512.)
+    // A one-tile item's second chain reads Q tile 0 as well.
     constexpr int kFmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
     constexpr int kFmtPv = kInt8 ? 0 : kFmt;
     constexpr uint32_t kIdescQk = umma_idesc_f16(kFmt, kBM, kBN, 0);
@@ -496,108 +534,126 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     const Desc q_desc(umma_smem_desc_sw128(smem_u32(q_smem), 16, 1024));
     const Desc ring_k(umma_smem_desc_sw128(smem_u32(k_ring), 16, 1024));
     const Desc ring_v(umma_smem_desc_sw128(smem_u32(v_ring), kBoxBytes, 1024));
-    auto commit = [&](uint64_t* bar) {
-      if (leader) umma_commit(bar);
-    };
     int base = 0;                   // key tiles of earlier segments
-    int q_waits[2] = {0, 0}, p_waits[2] = {0, 0};
+    int buf = 0, p_parity = 0;      // S buffer of the next step, and the phase of its P
+    int q_waits0 = 0, q_waits1 = 0;
     bool ok = true, issued_any = false;
-    auto wait_tile = [&](uint64_t* full, int slots, int i) {
-      return __all_sync(0xffffffffu, mbar_wait(full + i % slots, (i / slots) & 1, guard));
-    };
     walk.start(a, sh->share);
     while (ok && walk.next(a, s)) {
       if (s.tiles == 0) continue;
       issued_any = true;
-      const int steps = max(s.count[0], s.count[1]);
-      // Q K^T of chain c's step j; frees what its last reader is.
-      auto issue_qk = [&](int c, int j) -> bool {
-        const int entry = base + s.place(c, j);
-        if (!wait_tile(sh->k_full, kKSlots, entry)) return false;
-        tc_fence_after();
-        const int slot = entry % kKSlots;
-        const int q_tile = s.dual ? 0 : c;
-        if (leader) {
-          const Desc qd = q_desc.at(q_tile * kTileBytes);
-          const Desc kd = ring_k.at(slot * kTileBytes);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            umma_ss(tmem + c * 128, qd.at(kmajor_step(kk)).u64(), kd.at(kmajor_step(kk)).u64(),
-                    kIdescQk, kk > 0);
-          umma_commit(&sh->s_full[c]);
-        }
-        if (s.dual || c == 1) commit(&sh->k_empty[slot]);
-        // The chain's last Q K^T (of both chains for a shared Q tile: the one issued last).
-        if (s.dual ? s.place(c, j) + 1 == s.t1 - s.t0 : j + 1 == s.count[c])
-          commit(&sh->q_free[q_tile]);
-        return true;
+      const int steps = s.count0 + s.count1;
+      const int paired = s.dual ? steps : 2 * s.count0;   // steps in which the chains take turns
+      const int firsts = s.count0 > 0 ? 2 : 1;              // the chains' first steps are i < firsts
+      const int last0 = s.dual ? steps - 2 : paired - 2;    // a chain's last step, as is the last one
+      auto chain = [&](int i) { return i < paired ? i & 1 : 1; };
+      auto entry_of = [&](int i) {                          // Segment::place, from the first tile on
+        return base + (i < paired ? (s.dual ? i : i >> 1) : i - s.count0);
       };
-      for (int c = 0; c < 2 && ok; ++c) {
-        if (s.count[c] == 0) continue;
-        if (!s.dual || c == 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh->q_full[c], q_waits[c] & 1, guard));
-          if (!ok) break;
-          ++q_waits[c];
+      // Q K^T of step i once its K tile is there; frees what it is the last reader of.
+      auto issue_qk = [&](int i, int to) {
+        const int c = chain(i), q_tile = s.dual ? 0 : c, slot = entry_of(i) % kKSlots;
+        const Desc qd = q_desc.at(q_tile * kTileBytes);
+        const Desc kd = ring_k.at(slot * kTileBytes);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_ss(tmem + to * 128, qd.at(kmajor_step(kk)).u64(), kd.at(kmajor_step(kk)).u64(),
+                  kIdescQk, kk > 0);
+        umma_commit(&sh->s_full[to]);
+        if (s.dual || c == 1) umma_commit(&sh->k_empty[slot]);
+        if (i == steps - 1 || (!s.dual && i == last0)) umma_commit(&sh->q_free[q_tile]);
+      };
+      auto wait_k = [&](int i) {
+        const int entry = entry_of(i);
+        return mbar_wait(&sh->k_full[entry % kKSlots], (entry / kKSlots) & 1, guard);
+      };
+      auto wait_v = [&](int entry) {
+        return mbar_wait(&sh->v_full[entry % kVSlots], (entry / kVSlots) & 1, guard);
+      };
+      if (leader) {
+        for (int i = 0; ok && i < kSBufs && i < steps; ++i) {
+          const int c = chain(i);
+          if (i < firsts && !(s.dual && c == 1)) {
+            ok = mbar_wait(&sh->q_full[c], (c == 0 ? q_waits0 : q_waits1) & 1, guard);
+            ++(c == 0 ? q_waits0 : q_waits1);
+          }
+          ok = ok && wait_k(i);
+          tc_fence_after();
+          if (ok) issue_qk(i, (buf + i) % kSBufs);
         }
-        ok = issue_qk(c, 0);
       }
+      __syncwarp();
       int zeroed = -1;              // last V entry whose rows past the length were zeroed
-      for (int j = 0; j < steps && ok; ++j) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (!ok) break;
-          if (j < s.count[c]) {
-            const int entry = base + s.place(c, j);
-            const int slot = entry % kVSlots;
-            ok = wait_tile(sh->v_full, kVSlots, entry);
-            if (!ok) break;
-            if constexpr (!kInt8) {
-              const int keys = s.seq.len - s.tile(c, j) * kBN;   // of this tile
-              if (keys < kBN && zeroed != entry) {
-                zeroed = entry;
-                uint8_t* v = v_ring + slot * kTileBytes;
-                for (int i = lane; i < (kBN - keys) * 8 * G::kBoxes; i += 32) {
-                  const int row = keys + i / (8 * G::kBoxes), chunk = i % (8 * G::kBoxes);
-                  *reinterpret_cast<uint4*>(v + (chunk >> 3) * kBoxBytes + row * 128 +
-                                            (chunk & 7) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async_shared();
-                __syncwarp();
-              }
+      for (int i = 0; i < steps; ++i) {
+        const int c = chain(i), entry = entry_of(i), slot = entry % kVSlots;
+        if constexpr (!kInt8) {
+          const int keys = s.seq.len - (s.t0 + entry - base) * kBN;   // of this tile
+          if (keys < kBN && zeroed != entry) {
+            zeroed = entry;
+            if (leader) ok = ok && wait_v(entry);
+            __syncwarp();
+            uint8_t* v = v_ring + slot * kTileBytes;
+            for (int x = lane; x < (kBN - keys) * 8 * G::kBoxes; x += 32) {
+              const int row = keys + x / (8 * G::kBoxes), chunk = x % (8 * G::kBoxes);
+              *reinterpret_cast<uint4*>(v + (chunk >> 3) * kBoxBytes + row * 128 +
+                                        (chunk & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              ok = __all_sync(0xffffffffu, mbar_wait(&sh->p_half[c][half], p_waits[c] & 1, guard));
-              if (!ok) break;
-              tc_fence_after();
-              if (leader) {
-                const Desc vd = ring_v.at(slot * kTileBytes);
-#pragma unroll
-                for (int kq = 0; kq < kBN / 32; ++kq) {
-                  const int kk = half * (kBN / 32) + kq;
-                  umma_ts(tmem + 256 + c * 128, tmem + c * 128 + kk * 8,
-                          vd.at(mnmajor_step(kk)).u64(), kIdescPv, (j > 0 || kk > 0) ? 1u : 0u);
-                }
-              }
-            }
-            if (!ok) break;
-            ++p_waits[c];
-            if (s.dual) commit(&sh->v_empty[slot]);
-          }
-          // A two-tile item's V is read last by chain 1, whose tiles are the segment's.
-          if (!s.dual && c == 1) commit(&sh->v_empty[(base + j) % kVSlots]);
-          if (j + 1 < s.count[c]) {
-            ok = issue_qk(c, j + 1);
-          } else if (j + 1 == s.count[c]) {
-            commit(&sh->o_full[c]);
+            fence_proxy_async_shared();
+            __syncwarp();
           }
         }
+        if (leader && ok) {
+          const Desc vd = ring_v.at(slot * kTileBytes);
+          const uint32_t accumulate = i >= firsts;
+          auto issue_pv = [&](int half) {
+#pragma unroll
+            for (int kq = 0; kq < kBN / 32; ++kq) {
+              const int kk = half * (kBN / 32) + kq;
+              umma_ts(tmem + G::kOCol + c * D, tmem + buf * 128 + kk * 8,
+                      vd.at(mnmajor_step(kk)).u64(), kIdescPv, kk > 0 ? 1u : accumulate);
+            }
+          };
+          // What the step needs is asked for at once and waited for only where it is missing: four waits
+          // in a row cost 100 clocks each when everything is there, which is the usual case.
+          const int next = i + kSBufs;   // the step that takes this one's S buffer
+          const int next_entry = entry_of(next);
+          const bool k_ready = mbar_test_wait(&sh->k_full[next_entry % kKSlots],
+                                              (next_entry / kKSlots) & 1);
+          const bool v_ready = mbar_test_wait(&sh->v_full[slot], (entry / kVSlots) & 1);
+          const bool p0_ready = mbar_test_wait(&sh->p_half[buf][0], p_parity);
+          const bool p1_ready = mbar_test_wait(&sh->p_half[buf][1], p_parity);
+          ok = (v_ready || wait_v(entry)) &&
+               (p0_ready || mbar_wait(&sh->p_half[buf][0], p_parity, guard));
+          if (ok) {
+            tc_fence_after();
+            issue_pv(0);
+            if (!p1_ready) {
+              ok = mbar_wait(&sh->p_half[buf][1], p_parity, guard);
+              tc_fence_after();
+            }
+          }
+          if (ok) {
+            issue_pv(1);
+            // A two-tile item's V is read last by chain 1, whose tiles are the segment's.
+            if (s.dual || c == 1) umma_commit(&sh->v_empty[slot]);
+            if (i == last0 || i == steps - 1) umma_commit(&sh->o_full[c]);
+            if (next < steps) {
+              ok = k_ready || wait_k(next);
+              if (ok) issue_qk(next, buf);
+            }
+          }
+        }
+        if (++buf == kSBufs) {
+          buf = 0;
+          p_parity ^= 1;
+        }
       }
+      ok = __all_sync(0xffffffffu, ok);
       base += s.t1 - s.t0;
     }
     // Every MMA issued has completed before TMEM may be released.
     if (issued_any) {
-      commit(&sh->mma_done);
+      if (leader) umma_commit(&sh->mma_done);
       mbar_wait(&sh->mma_done, 0, guard);
     }
   } else if (warp < kProducerWarp) {
@@ -607,12 +663,12 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     const int quarter = warp & 3;             // TMEM lane quarter this warp may access
     const int row = quarter * 32 + lane;      // of the tile
     const uint32_t lane_field = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t taddr_s = tmem + c * 128 + lane_field;
-    const uint32_t taddr_o = tmem + 256 + c * 128 + lane_field;
+    const uint32_t taddr_o = tmem + G::kOCol + c * D + lane_field;
     const int row_token = row / a.group;
     const int row_head = row - row_token * a.group;
-    int s_waits = 0, o_waits[2] = {0, 0}, joins = 0;
-    int kv_base = 0;                          // key tiles of earlier segments (int8: scale slots)
+    int n_base = 0;                           // steps of earlier segments
+    int o_waits = 0, joins = 0;
+    int kv_base = 0;                          // key tiles of earlier segments
     int segments = 0;
     int4 meta0 = make_int4(0, 0, 0, 0), meta1 = make_int4(0, 0, 0, 0);
     bool ok = true;
@@ -627,23 +683,27 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
       const bool warp_ok = quarter * 32 < tile_rows;     // some row of this warp holds a token
       const int offset = s.seq.len - s.seq.n + s.first;  // position of the item's first token
       const int limit = a.causal ? min(s.seq.len, offset + token + 1) : s.seq.len;
-      const int count = s.count[c];
+      const int count = s.count(c);
 
       float m_ref = -INFINITY;  // log2-domain reference point of this row
       float l_sum = 0.f;
       for (int j = 0; j < count; ++j) {
-        if (!mbar_wait(&sh->s_full[c], s_waits & 1, guard)) {
+        const int n = n_base + s.order(c, j), buf = n % kSBufs;
+        if (!mbar_wait(&sh->s_full[buf], (n / kSBufs) & 1, guard)) {
           ok = false;
           break;
         }
-        ++s_waits;
         if (!warp_ok) {   // whatever P holds stays in rows that nobody reads
           tc_fence_after();
           tc_fence_before();
-          mbar_arrive(&sh->p_half[c][0]);
-          mbar_arrive(&sh->p_half[c][1]);
+          mbar_arrive(&sh->p_half[buf][0]);
+          mbar_arrive(&sh->p_half[buf][1]);
           continue;
         }
+        const uint32_t taddr_s = tmem + buf * 128 + lane_field;
+        const int v_prev = kv_base + (j > 0 ? s.place(c, j - 1) : 0);
+        const PrevPv prev{&sh->v_empty[v_prev % kVSlots],
+                          static_cast<uint32_t>((v_prev / kVSlots) & 1)};
         tc_fence_after();
         const int k0 = s.tile(c, j) * kBN;
         const bool masked = k0 + kBN > s.seq.len ||
@@ -657,20 +717,21 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
           const float* scales = reinterpret_cast<const float*>(smem + G::kScaleOffset) +
                                 (at % G::kScaleSlots) * 3 * kBN;
           softmax_tile_int8<D>(taddr_s, taddr_o, scales, masked, limit - k0, m_ref, l_sum,
-                               sh->p_half[c]);
+                               sh->p_half[buf], prev, guard);
         } else {
           softmax_tile<T, D>(taddr_s, taddr_o, a.scale_log2, masked, limit - k0, m_ref, l_sum,
-                             sh->p_half[c]);
+                             sh->p_half[buf], prev, guard);
         }
       }
       if (!ok) break;
       kv_base += s.t1 - s.t0;
+      n_base += s.count0 + s.count1;
 
       // The end of the segment. Its O is read before this warpgroup publishes the next segment's
       // first P, which the first P V that overwrites O waits for.
       if (count > 0) {
-        if (!mbar_wait(&sh->o_full[c], o_waits[c] & 1, guard)) break;
-        ++o_waits[c];
+        if (!mbar_wait(&sh->o_full[c], o_waits & 1, guard)) break;
+        ++o_waits;
       }
       float m_other = -INFINITY, l_other = 0.f;
       if (s.dual) {
@@ -690,7 +751,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
         l_other = ml.y;
       }
       tc_fence_after();
-      const bool join = s.count[1] > 0 && s.dual;
+      const bool join = s.count1 > 0 && s.dual;
       const float m = fmaxf(m_ref, m_other);
       const float ref = m == -INFINITY ? 0.f : m;
       float f0 = ex2(m_ref - ref), f1 = ex2(m_other - ref);
@@ -725,7 +786,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
           for (int e = 0; e < 32; ++e) of[e] *= f0;
           if (join) {
             uint32_t ow[32];
-            tmem_ld32(taddr_o + 128 + i * 32, ow);
+            tmem_ld32(taddr_o + D + i * 32, ow);
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 32; ++e) of[e] = fmaf(__uint_as_float(ow[e]), f1, of[e]);
@@ -990,7 +1051,7 @@ int launch(const ExtendArgs& a, const CUtensorMap& tmq, const CUtensorMap& tmk,
            const CUtensorMap& tmv, int ctas, int dev, cudaStream_t stream) {
   using G = Geometry<D, kInt8>;
   constexpr int kSmem = G::kTailOffset + static_cast<int>(sizeof(Shared<G::kKSlots, G::kVSlots, G::kCodeSlots,
-                                                               G::kScaleSlots>)) +
+                                                               G::kScaleSlots, G::kSBufs>)) +
                         1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
   auto kernel = extend_kernel<T, D, kInt8>;

@@ -108,12 +108,19 @@ struct Segment {
   int b, hkv, first, tokens;   // sequence, KV head, first token in it, tokens
   int t0, t1, tiles;
   bool dual;                   // the tokens fit in one tile
-  int count[2];                // key tiles each chain runs here
+  int count0, count1;          // key tiles each chain runs here
+
+  __device__ __forceinline__ int count(int c) const { return c == 0 ? count0 : count1; }
 
   // Chain c's j-th key tile.
   __device__ __forceinline__ int tile(int c, int j) const { return dual ? t0 + 2 * j + c : t0 + j; }
   // Its place among the segment's key tiles.
   __device__ __forceinline__ int place(int c, int j) const { return dual ? 2 * j + c : j; }
+  // The chains take turns while both have steps (chain 0 runs out first in a two-tile item): the
+  // place of chain c's j-th step among the steps of both.
+  __device__ __forceinline__ int order(int c, int j) const {
+    return dual || j < count0 ? 2 * j + c : count0 + j;
+  }
 };
 
 // Where a CTA's share starts (unit `at` of item k of a sequence and KV head) and its length.
@@ -176,11 +183,11 @@ struct Walk {
       if (s.t1 > s.t0 || (s.tiles == 0 && from == 0)) {
         const int n = s.t1 - s.t0;
         if (s.dual) {
-          s.count[0] = (n + 1) / 2;
-          s.count[1] = n / 2;
+          s.count0 = (n + 1) / 2;
+          s.count1 = n / 2;
         } else {
-          s.count[0] = min(max(tiles_seen(a, s.seq, s.first + a.tile_tokens), s.t0), s.t1) - s.t0;
-          s.count[1] = n;
+          s.count0 = min(max(tiles_seen(a, s.seq, s.first + a.tile_tokens), s.t0), s.t1) - s.t0;
+          s.count1 = n;
         }
         return true;
       }

@@ -269,9 +269,10 @@ def extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seq_le
     Returns o in q's shape and dtype and, with return_lse=True, the natural-log log-sum-exp of
     each score row as fp32 in q's shape without its last dimension. Rows that see no key, or
     belong to no sequence, give zeros and -inf. One call takes at most 16384 sequences and 128
-    query heads per KV head. A non-finite value in V makes the whole tile of up to 128 keys around it non-finite for every row that reads the tile, also for rows that the
-    causal mask keeps from that key (int8 caches: only for the rows that see it); keys at or past
-    seq_lens[b] are never read into a result.
+    query heads per KV head. A non-finite value in V makes the whole tile of up to 128 keys around
+    it non-finite for every row that reads the tile, also for rows that the causal mask keeps from
+    that key (int8 caches: only for the rows that see it); keys at or past seq_lens[b] are never
+    read into a result.
     """
     out, lse = _extend_checked(0, q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, causal,
                                softmax_scale, k_scale, v_scale)
