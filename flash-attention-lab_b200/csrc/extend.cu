@@ -184,10 +184,13 @@ __device__ __forceinline__ void convert_tile(const uint8_t* codes, uint8_t* tile
 // --------------------------------------------------------------------------------------------
 
 // The barrier phase by which P V of a chain's previous step has completed: the release of its V tile
-// (in a two-tile item by chain 1's P V, which does not wait for this step of either chain).
+// (in a two-tile item by chain 1's P V, which does not wait for this step of either chain). `needed`
+// when this step's scores do not say so, that is when fewer than kSBufs steps lie between: only then
+// is the phase sure to be the barrier's current or last one, whatever the number of V slots.
 struct PrevPv {
   uint64_t* bar;
   uint32_t parity;
+  bool needed;
 };
 
 // The reference point of a row moves only when its maximum mt (log2 domain) passes it by more than
@@ -204,8 +207,10 @@ __device__ __forceinline__ void move_reference(float mt, float& m_ref, float& l_
   if (rescale) l_sum *= factor;
   m_ref = m_new;
   if (__any_sync(0xffffffffu, rescale)) {
-    if (!mbar_wait(prev.bar, prev.parity, guard)) return;   // the next wait gives up as well
-    tc_fence_after();
+    if (prev.needed) {
+      if (!mbar_wait(prev.bar, prev.parity, guard)) return;   // the next wait gives up as well
+      tc_fence_after();
+    }
 #pragma unroll 1
     for (int i = 0; i < D / 16; ++i) {
       uint32_t ov[16];
@@ -703,7 +708,8 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
         const uint32_t taddr_s = tmem + buf * 128 + lane_field;
         const int v_prev = kv_base + (j > 0 ? s.place(c, j - 1) : 0);
         const PrevPv prev{&sh->v_empty[v_prev % kVSlots],
-                          static_cast<uint32_t>((v_prev / kVSlots) & 1)};
+                          static_cast<uint32_t>((v_prev / kVSlots) & 1),
+                          j > 0 && s.order(c, j) - s.order(c, j - 1) < kSBufs};
         tc_fence_after();
         const int k0 = s.tile(c, j) * kBN;
         const bool masked = k0 + kBN > s.seq.len ||

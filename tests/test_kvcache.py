@@ -304,6 +304,27 @@ def test_extend_scales(scale, int8):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True], ids=["16bit", "int8"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [20, 160])
+def test_extend_scores_that_grow_along_the_keys(new, d, int8):
+    # The reference point of nearly every row moves at every key tile, in items of one tile (20
+    # tokens) and of two, by several tiles of one CTA: 2 x 8 x about 30 of them for 148 CTAs.
+    lens = [4500, 3400]
+    cache = Cache(lens, 8, d, torch.bfloat16, int8)
+    factor = 6.0 * (torch.arange(cache.rows, device="cuda") // 128 + 1)
+    if int8:
+        cache.scales["k_scale"] *= factor[None, :, None]
+        steps = np.concatenate([host64(cache.scales["k_scale"][b, :n]) for b, n in enumerate(lens)])
+        codes = np.concatenate([host64(cache.k[b, :n]) for b, n in enumerate(lens)])
+        cache.host["k"] = codes * steps[..., None]
+    else:
+        cache.k *= factor[None, :, None, None].to(torch.bfloat16)
+        cache.host["k"] = np.concatenate([host64(cache.k[b, :n]) for b, n in enumerate(lens)])
+    check_extend(cache, [new, new], 16, torch.bfloat16)
+
+
+@pytest.mark.gpu
 def test_extend_int8_scales_of_any_size():
     # V rows of very different sizes, tiny and zero rows among them: the weights carry the scales.
     cache = Cache([300], 1, 64, torch.bfloat16, True)
