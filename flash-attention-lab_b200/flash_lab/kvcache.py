@@ -196,6 +196,11 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         return
     shape = check_cache_inputs(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale,
                                cu_seqlens, {"k": k, "v": v})
+    for name, x in (("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale),
+                    ("v_scale", v_scale)):
+        if x is not None and any(n > 1 and st == 0 for n, st in zip(x.shape, x.stride())):
+            raise ValueError(f"{name} is written and must not be expanded, got strides "
+                             f"{tuple(x.stride())} for shape {tuple(x.shape)}")
     if k.shape != v.shape:
         raise ValueError(f"k and v must have the same shape, got {tuple(k.shape)} and "
                          f"{tuple(v.shape)}")

@@ -839,6 +839,18 @@ def test_int8_cache_refusals():
         flash_lab.decode(q, kc, vc, lens, k_scale=scale, v_scale=scale)
 
 
+def test_append_refuses_expanded_caches():
+    # Sequences (or heads, for scales) that share memory would be written by several threads at once.
+    kc, vc, lens = cpu_args()
+    k = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="k_cache is written"):
+        flash_lab.append_kv(k, k, kc[:1].expand(2, -1, -1, -1), vc, lens)
+    scale = torch.ones(2, 16, 2)
+    with pytest.raises(ValueError, match="v_scale is written"):
+        flash_lab.append_kv(k, k, kc.to(torch.int8), vc.to(torch.int8), lens, k_scale=scale,
+                            v_scale=scale[..., :1].expand(-1, -1, 2))
+
+
 def test_append_and_gather_refusals():
     kc, vc, lens = cpu_args()
     k = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
