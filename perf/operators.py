@@ -224,18 +224,13 @@ def run(state):
     return _own(state) if own else _plain(state)
 
 
-_module = None
-
-
 def _flash_lab():
-    """The package, imported by the first pass as a user's program imports it once."""
-    global _module
-    if _module is None:
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
-                                        "flash-attention-lab_b200"))
-        import flash_lab
-        _module = flash_lab
-    return _module
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                        "flash-attention-lab_b200")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import flash_lab
+    return flash_lab
 
 
 def _own(s):
