@@ -110,7 +110,7 @@ struct Shared {
   uint64_t s_full[kSBufs];
   uint64_t p_half[kSBufs][2];   // P of keys 0-63 / 64-127 of a tile stored in TMEM
   uint64_t o_full[2];
-  uint64_t x_ready, x_done;  // joining the two chains of a one-tile item
+  uint64_t x_ready, x_done;  // the chains' meeting at the end of a joined segment
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort_flag;
@@ -553,10 +553,10 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
       if (s.tiles == 0) continue;
       issued_any = true;
       const int steps = s.count0 + s.count1;
-      const int paired = s.dual ? steps : 2 * s.count0;   // steps in which the chains take turns
+      const int paired = s.paired();
       const int firsts = s.count0 > 0 ? 2 : 1;              // the chains' first steps are i < firsts
-      const int last0 = s.dual ? steps - 2 : paired - 2;    // a chain's last step, as is the last one
-      auto chain = [&](int i) { return i < paired ? i & 1 : 1; };
+      const int last0 = s.other_last();                     // a chain's last step, as is the last one
+      auto chain = [&](int i) { return s.chain(i); };
       auto entry_of = [&](int i) {                          // Segment::place, from the first tile on
         return base + (i < paired ? (s.dual ? i : i >> 1) : i - s.count0);
       };
@@ -745,8 +745,10 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
         ++o_waits;
       }
       float m_other = -INFINITY, l_other = 0.f;
-      if (s.dual) {
-        // Chain 1 hands its (m, l) to chain 0, which reads both O and writes the joint result.
+      if (s.joined()) {
+        // Chain 1 hands its (m, l) to chain 0, which reads both O and writes the joint result. In an
+        // item whose first tile sees no key here the chains only meet: chain 0, which has had no
+        // step to wait for, must not reach the next items' barriers ahead of these steps.
         const uint32_t phase = joins++ & 1;
         if (c == 1) {
           sh->x_ml[row] = make_float2(m_ref, l_sum);
@@ -754,12 +756,17 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
           mbar_arrive(&sh->x_ready);
           if (!mbar_wait(&sh->x_done, phase, guard)) break;
           tc_fence_after();
-          continue;
+          if (s.dual) continue;
+        } else {
+          if (!mbar_wait(&sh->x_ready, phase, guard)) break;
+          if (s.dual) {
+            const float2 ml = sh->x_ml[row];
+            m_other = ml.x;
+            l_other = ml.y;
+          } else {
+            mbar_arrive(&sh->x_done);
+          }
         }
-        if (!mbar_wait(&sh->x_ready, phase, guard)) break;
-        const float2 ml = sh->x_ml[row];
-        m_other = ml.x;
-        l_other = ml.y;
       }
       tc_fence_after();
       const bool join = s.count1 > 0 && s.dual;

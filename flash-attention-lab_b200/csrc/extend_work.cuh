@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "extend_steps.h"
 #include "kv_cache.cuh"
 #include "sm100.cuh"
 
@@ -102,25 +103,14 @@ __device__ __forceinline__ int item_units(const ExtendArgs& a, const Sequence& s
   return kItemUnits + weight * tiles_seen(a, s, last);
 }
 
-// A CTA's part of an item: key tiles [t0, t1) of all `tiles`.
-struct Segment {
+// A CTA's part of an item: key tiles [t0, t1) of all `tiles`. dual: the tokens fit in one tile.
+struct Segment : Steps {
   Sequence seq;
   int b, hkv, first, tokens;   // sequence, KV head, first token in it, tokens
   int t0, t1, tiles;
-  bool dual;                   // the tokens fit in one tile
-  int count0, count1;          // key tiles each chain runs here
-
-  __device__ __forceinline__ int count(int c) const { return c == 0 ? count0 : count1; }
 
   // Chain c's j-th key tile.
-  __device__ __forceinline__ int tile(int c, int j) const { return dual ? t0 + 2 * j + c : t0 + j; }
-  // Its place among the segment's key tiles.
-  __device__ __forceinline__ int place(int c, int j) const { return dual ? 2 * j + c : j; }
-  // The chains take turns while both have steps (chain 0 runs out first in a two-tile item): the
-  // place of chain c's j-th step among the steps of both.
-  __device__ __forceinline__ int order(int c, int j) const {
-    return dual || j < count0 ? 2 * j + c : count0 + j;
-  }
+  __device__ __forceinline__ int tile(int c, int j) const { return t0 + place(c, j); }
 };
 
 // Where a CTA's share starts (unit `at` of item k of a sequence and KV head) and its length.
