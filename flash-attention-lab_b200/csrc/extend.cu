@@ -853,8 +853,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kOtherRegs));
     if constexpr (kInt8) {
       // ------------------------------- code converters -------------------------------
-      // One warpgroup for K, one for V. Code tiles arrive in the producer's order: of a segment's n
-      // key tiles K 0, K 1, V 0, K 2, V 1, ..., V n - 1.
+      // One warpgroup for K, one for V. Code tiles are copied in the producer's order (code_place).
       const bool is_v = warp >= kConvertWarp + 4;
       const int tid = threadIdx.x - (is_v ? kConvertWarp + 4 : kConvertWarp) * 32;
       const bool paged = a.cache.block_tables != nullptr;
@@ -862,13 +861,16 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
       bool ok = true;
       // Key tile i of the segment, once it and its place in the 16-bit ring are there.
       auto convert = [&](int i, int n) -> bool {
-        const int code = 2 * base + (is_v ? (i + 1 < n ? 2 * i + 2 : 2 * i + 1) : max(2 * i - 1, 0));
-        const int code_slot = code % G::kCodeSlots;
+        const int code = 2 * base + code_place(is_v, i, n);
+        const int code_slot = code % G::kCodeSlots, code_phase = code / G::kCodeSlots;
+        // The place's last tile may have been the other warpgroup's: its release says that the phase
+        // of code_full before this one has completed.
+        if (code_phase > 0 && !mbar_wait(&sh->code_empty[code_slot], (code_phase - 1) & 1, guard))
+          return false;
+        if (!mbar_wait(&sh->code_full[code_slot], code_phase & 1, guard)) return false;
         const int at = base + i, slots = is_v ? kVSlots : kKSlots, slot = at % slots;
         uint64_t* empty = is_v ? &sh->v_empty[slot] : &sh->k_empty[slot];
-        if (!mbar_wait(&sh->code_full[code_slot], (code / G::kCodeSlots) & 1, guard) ||
-            (at >= slots && !mbar_wait(empty, ((at / slots) - 1) & 1, guard)))
-          return false;
+        if (at >= slots && !mbar_wait(empty, ((at / slots) - 1) & 1, guard)) return false;
         const uint8_t* codes = smem + G::kCodeOffset + code_slot * G::kCodeBytes;
         if (is_v) {
           convert_tile<__half, D>(codes, v_ring + slot * kTileBytes, tid);

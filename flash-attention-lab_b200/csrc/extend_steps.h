@@ -20,6 +20,10 @@
 //   x_ready/done  Once per joined segment, waited for each time by the other chain.
 //   q, k, v       Rings whose two sides wait for every phase. A chain also waits for the v_empty of its
 //                 previous step's tile, see PrevPv.
+//   code_full[s]  The tiles of one place belong to K and V by turns, and copies land in any order: a
+//                 converter that waits for its tile knows nothing of the one before, which is the
+//                 other's. So it waits for that tile's release first. Its own comes next, so the
+//                 release cannot be a phase further.
 #pragma once
 
 #ifdef __CUDACC__
@@ -52,5 +56,11 @@ struct Steps {
   // The chains meet at the segment's end.
   FLB_HD bool joined() const { return dual || count0 == 0; }
 };
+
+// Place of the i-th K or V tile of codes among the 2 n of a segment, in the producer's order: K 0,
+// K 1, V 0, K 2, V 1, ..., V n - 1.
+FLB_HD int code_place(bool is_v, int i, int n) {
+  return is_v ? (i + 1 < n ? 2 * i + 2 : 2 * i + 1) : (i > 0 ? 2 * i - 1 : 0);
+}
 
 }  // namespace flb

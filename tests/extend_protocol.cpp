@@ -1,10 +1,11 @@
-// Host model of extend_kernel's barriers between the MMA lane, the tensor cores and the two softmax
-// warpgroups, on the step order of csrc/extend_steps.h: every interleaving of the roles over sequences
-// of segments. A wait passes by parity, as mbarrier.try_wait.parity does; a role that waits
+// Host model of extend_kernel's barriers, on the step order of csrc/extend_steps.h: between the MMA lane,
+// the tensor cores and the two softmax warpgroups, and between the producer, its copies and the two
+// converters of codes. Every interleaving of the roles over sequences of segments. A wait passes by parity, as mbarrier.try_wait.parity does; a role that waits
 // while its phase is two ahead (the wait would pass early) or two behind (it would block for good) is a
 // violation, and so is a state from which no role can go on.
 //
 //   extend_protocol softmax RULE    RULE joined: as the kernel; dual: only one-tile segments joined
+//   extend_protocol codes RULE      RULE release: as the kernel; full: converters wait for code_full alone
 //
 // Prints the number of sequences and of states, or the first violation (exit 1).
 #include <cstdint>
@@ -61,7 +62,16 @@ Result explore(const Model& m) {
   Result result;
   std::unordered_set<uint64_t> seen{0};
   std::vector<uint64_t> todo{0};
-  auto place = [](uint64_t s, size_t r) { return static_cast<size_t>(s >> (12 * r)) & 0xfff; };
+  const size_t bits = 64 / roles;
+  for (const Program& program : m.roles) {
+    if (program.size() >> bits != 0) {
+      result.error = "a program is too long for the state";
+      return result;
+    }
+  }
+  auto place = [&](uint64_t s, size_t r) {
+    return static_cast<size_t>(s >> (bits * r)) & ((size_t{1} << bits) - 1);
+  };
   while (!todo.empty()) {
     const uint64_t s = todo.back();
     todo.pop_back();
@@ -86,7 +96,7 @@ Result explore(const Model& m) {
         if (completed == op.phase) continue;
       }
       moved = true;
-      const uint64_t next = s + (uint64_t{1} << (12 * r));
+      const uint64_t next = s + (uint64_t{1} << (bits * r));
       if (seen.insert(next).second) todo.push_back(next);
     }
     if (!moved && !ended) {
@@ -205,6 +215,49 @@ bool softmax(bool join_count0) {
   return true;
 }
 
+// Roles: 0 the producer, 1 and 2 the converters of K and V, then one for each place of the ring, whose
+// copies land at any time after their issue, in any order among places.
+Model codes_model(const std::vector<int>& tiles, int slots, bool wait_release) {
+  Model m;
+  m.roles.resize(3 + slots);
+  int base = 0;
+  for (int n : tiles) {
+    for (int code = 2 * base; code < 2 * (base + n); ++code) {
+      const int slot = code % slots, phase = code / slots;
+      if (phase > 0) m.wait(0, numbered("code_empty", slot), phase - 1);
+      m.arrive(0, numbered("copy", slot));
+      m.wait(3 + slot, numbered("copy", slot), phase);
+      m.arrive(3 + slot, numbered("code_full", slot));
+    }
+    for (int is_v = 0; is_v < 2; ++is_v) {
+      for (int i = 0; i < n; ++i) {
+        const int code = 2 * base + flb::code_place(is_v, i, n);
+        const int slot = code % slots, phase = code / slots;
+        if (wait_release && phase > 0) m.wait(1 + is_v, numbered("code_empty", slot), phase - 1);
+        m.wait(1 + is_v, numbered("code_full", slot), phase);
+        m.arrive(1 + is_v, numbered("code_empty", slot));
+      }
+    }
+    base += n;
+  }
+  return m;
+}
+
+bool codes(bool wait_release) {
+  for (int slots : {3, 6}) {   // head_dim 128 and 64
+    for (int a = 1; a <= 6; ++a) {
+      for (int b = 0; b <= 4; ++b) {
+        for (int c = 0; c <= 3; ++c) {
+          const std::string what = std::to_string(slots) + " places, segments of " + std::to_string(a) +
+                                   ", " + std::to_string(b) + ", " + std::to_string(c) + " tiles";
+          if (!check(codes_model({a, b, c}, slots, wait_release), what)) return false;
+        }
+      }
+    }
+  }
+  return true;
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -212,8 +265,10 @@ int main(int argc, char** argv) {
   bool ok;
   if (part == "softmax" && (rule == "joined" || rule == "dual")) {
     ok = softmax(rule == "joined");
+  } else if (part == "codes" && (rule == "release" || rule == "full")) {
+    ok = codes(rule == "release");
   } else {
-    std::printf("usage: extend_protocol softmax joined|dual\n");
+    std::printf("usage: extend_protocol softmax joined|dual, or codes release|full\n");
     return 2;
   }
   if (ok) std::printf("%ld sequences, %ld states\n", sequences, states);

@@ -33,3 +33,11 @@ def test_softmax_warpgroups_never_wait_for_a_phase_two_ahead(model):
     # The model sees the fault where only the items of one tile make the chains meet.
     code, text = model("softmax", "dual")
     assert code == 1 and "two-tile(0, 1) two-tile(0, 1)" in text and "s_full" in text
+
+
+def test_converters_never_wait_for_a_phase_two_ahead(model):
+    code, text = model("codes", "release")
+    assert code == 0, text
+    # A place's last tile may be the other converter's, and its copy the last to land.
+    code, text = model("codes", "full")
+    assert code == 1 and "3 places" in text and "code_full" in text
