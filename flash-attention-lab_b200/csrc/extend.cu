@@ -9,7 +9,8 @@
 // of K multiplies a column of S, and the scale of V joins the exponent,
 //     w_j = 2^(z_j - M),  z_j = s_j + log2 sv_j,  o = sum_j w_j V_j / sum_j (w_j / sv_j),
 // so the weights that enter the second product as fp16 lie in (0, 2^8] whatever the size of the
-// scales, and no rounding beyond theirs is made.
+// scales. Weights below 2^-25 are 0 there (N of them make o differ by less than N 2^-18 steps of the row
+// with the largest weight); the sum of w_j / sv_j in fp32 keeps them.
 //
 // What bounds it. Every K/V byte is read once per 2 x 128 rows, so few rows per sequence are bound
 // by HBM (2 H_kv D bytes per key at 8 bits, twice that at 16) and chunks of hundreds of rows by the
@@ -81,7 +82,11 @@ struct Geometry {
   // Key tiles whose scales are held: a K tile is converted once Q K^T of the tile kKSlots earlier
   // has been issued, which follows the softmax of tiles kSBufs or more before that one.
   static constexpr int kScaleSlots = kInt8 ? kKSlots + kSBufs : 0;
-  static constexpr int kScaleBytes = kScaleSlots * 3 * kBN * 4;
+  // mult, log2 sv and 1 / sv of each key; then, from each warp of 32 keys, a byte: whether the row sum
+  // needs care (softmax_tile_int8).
+  static constexpr int kCareAt = 3 * kBN;
+  static constexpr int kScaleWords = kCareAt + 4;
+  static constexpr int kScaleBytes = kScaleSlots * kScaleWords * 4;
   static constexpr int kRingOffset = 2 * kTileBytes;
   static constexpr int kCodeOffset = kRingOffset + kSlots * kTileBytes;
   static constexpr int kScaleOffset = kCodeOffset + kCodeSlots * kCodeBytes;
@@ -209,7 +214,7 @@ __device__ __forceinline__ void move_reference(float mt, float& m_ref, float& l_
   if (m_ref == -INFINITY || mt > m_ref + kRescaleThreshold) m_new = fmaxf(m_ref, mt);
   const bool rescale = (m_new != m_ref) && (m_ref != -INFINITY);
   const float factor = rescale ? ex2(m_ref - m_new) : 1.f;
-  if (rescale) l_sum *= factor;
+  if (rescale) l_sum = scale_sum(l_sum, m_ref - m_new);
   m_ref = m_new;
   if (__any_sync(0xffffffffu, rescale)) {
     if (prev.needed) {
@@ -286,10 +291,60 @@ __device__ __forceinline__ void softmax_tile(uint32_t taddr_s, uint32_t taddr_o,
   l_sum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
 }
 
+// The second pass over an int8 tile: weights from the scaled scores z in TMEM, and their sum over
+// w / sv. kWide: the sum's terms 2^(z - log2 sv - M) by exponentials of their own.
+template <bool kWide>
+__device__ __forceinline__ void weights_int8(uint32_t taddr_s, const float* scales, float nref,
+                                             float (&ps)[4], uint64_t* bars) {
+  constexpr int kCols = kWide ? 16 : 32;   // the rare form must not cost the usual one registers
+#pragma unroll 1
+  for (int c0 = 0; c0 < 128; c0 += kCols) {
+    uint32_t zr[kCols], pk[kCols / 2];
+    if constexpr (kWide) tmem_ld16(taddr_s + c0, zr);
+    else tmem_ld32(taddr_s + c0, zr);
+    tmem_ld_wait();
+    float* z = reinterpret_cast<float*>(zr);
+#pragma unroll
+    for (int i = 0; i < kCols; i += 4) {
+      const float4 by = *reinterpret_cast<const float4*>(scales + (kWide ? 1 : 2) * kBN + c0 + i);
+      float p[4];
+      fadd2(p[0], p[1], z[i], z[i + 1], nref, nref);
+      fadd2(p[2], p[3], z[i + 2], z[i + 3], nref, nref);
+      if constexpr (kWide) {
+        const float r[4] = {by.x, by.y, by.z, by.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // The square of a root: the term may be below the exponential's range, 2^-126. Keys past
+          // the length: log2 sv is -inf.
+          const float root = ex2(0.5f * (p[e] - r[e]));
+          ps[e] = r[e] == -INFINITY ? ps[e] : fmaf(root, root, ps[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = ex2(p[e]);
+      if constexpr (!kWide) {
+        ffma2(ps[0], ps[1], p[0], p[1], by.x, by.y, ps[0], ps[1]);
+        ffma2(ps[2], ps[3], p[2], p[3], by.z, by.w, ps[2], ps[3]);
+      }
+      pk[i / 2] = pack2<__half>(p[0], p[1]);
+      pk[i / 2 + 1] = pack2<__half>(p[2], p[3]);
+    }
+    if constexpr (kWide) tmem_st8(taddr_s + c0 / 2, pk);
+    else tmem_st16(taddr_s + c0 / 2, pk);
+    if (((c0 + kCols) & 63) == 0) publish_half(&bars[c0 / 64]);
+  }
+}
+
 // The same over an int8 cache, with fp16 weights. `scales` holds the tile's per-key numbers in shared
-// memory: mult, log2 sv and 1 / sv. They are read once: the scaled scores z go back to TMEM between
-// the two passes. 32 columns at a time leave registers to read ahead; with all 128 in registers the
+// memory: mult, log2 sv and 1 / sv. They are read once: the scaled scores z go back to TMEM between the
+// two passes. 32 columns at a time leave registers to read ahead; with all 128 in registers the
 // loop spilled, and the spills cost more than the softmax.
+//
+// A weight under 2^-126 is 0, and its term w / sv with it, however small sv is: a row of zeros in V has
+// sv = 2^-100. What a tile can lose that way is 128 terms under 2^-126 / sv, which is below 2^-32 of the
+// row's sum when the scales so far in the segment lie in [2^-40, 2^45] (a row that sees a key has a sum of
+// at least 1 / sv of one of them) or the sum is at least 2^13. Else the terms take exponentials of
+// their own.
 template <int D>
 __device__ __forceinline__ void softmax_tile_int8(uint32_t taddr_s, uint32_t taddr_o,
                                                   const float* scales, bool masked, int visible,
@@ -323,31 +378,17 @@ __device__ __forceinline__ void softmax_tile_int8(uint32_t taddr_s, uint32_t tad
     tmem_st32(taddr_s + c0, sr);
   }
   tmem_st_wait();
-  move_reference<D>(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), m_ref, l_sum, taddr_o, prev,
-                    guard);
+  const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+  move_reference<D>(mx, m_ref, l_sum, taddr_o, prev, guard);
   const float nref = m_ref == -INFINITY ? 0.f : -m_ref;
+  bool wide = false;
+  if (reinterpret_cast<const int*>(scales)[Geometry<D, true>::kCareAt] != 0)   // of all rows alike
+    wide = __any_sync(0xffffffffu, mx != -INFINITY && !(l_sum >= 0x1p13f));
   float ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-  for (int c0 = 0; c0 < 128; c0 += 32) {
-    uint32_t zr[32], pk[16];
-    tmem_ld32(taddr_s + c0, zr);
-    tmem_ld_wait();
-    float* z = reinterpret_cast<float*>(zr);
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 inv = *reinterpret_cast<const float4*>(scales + 2 * kBN + c0 + i);
-      float p[4];
-      fadd2(p[0], p[1], z[i], z[i + 1], nref, nref);
-      fadd2(p[2], p[3], z[i + 2], z[i + 3], nref, nref);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = ex2(p[e]);
-      ffma2(ps[0], ps[1], p[0], p[1], inv.x, inv.y, ps[0], ps[1]);
-      ffma2(ps[2], ps[3], p[2], p[3], inv.z, inv.w, ps[2], ps[3]);
-      pk[i / 2] = pack2<__half>(p[0], p[1]);
-      pk[i / 2 + 1] = pack2<__half>(p[2], p[3]);
-    }
-    tmem_st16(taddr_s + c0 / 2, pk);
-    if (c0 & 32) publish_half(&bars[c0 / 64]);
+  if (wide) {
+    weights_int8<true>(taddr_s, scales, nref, ps, bars);
+  } else {
+    weights_int8<false>(taddr_s, scales, nref, ps, bars);
   }
   l_sum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
 }
@@ -726,7 +767,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
             break;
           }
           const float* scales = reinterpret_cast<const float*>(smem + G::kScaleOffset) +
-                                (at % G::kScaleSlots) * 3 * kBN;
+                                (at % G::kScaleSlots) * G::kScaleWords;
           softmax_tile_int8<D>(taddr_s, taddr_o, scales, masked, limit - k0, m_ref, l_sum,
                                sh->p_half[buf], prev, guard);
         } else {
@@ -774,7 +815,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
       const float ref = m == -INFINITY ? 0.f : m;
       float f0 = ex2(m_ref - ref), f1 = ex2(m_other - ref);
       if (!s.dual) f0 = 1.f;
-      const float l = s.dual ? l_sum * f0 + l_other * f1 : l_sum;
+      const float l = s.dual ? scale_sum(l_sum, m_ref - ref) + scale_sum(l_other, m_other - ref) : l_sum;
       const bool whole = s.t0 == 0 && s.t1 == s.tiles;
       if (whole) {
         // A row that saw nothing has l = 0; a NaN sum stays NaN.
@@ -913,6 +954,7 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
         };
         float sk = 0.f, sv = 0.f;
         int blk_next = 0;
+        bool care = false;   // these keys of the segment had a V scale out of the ordinary
         if (n > 0) {
           scales_of(s.t0, block_of(s.t0), sk, sv);
           blk_next = block_of(s.t0 + 1);
@@ -931,16 +973,19 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
             break;
           }
           float* out = reinterpret_cast<float*>(smem + G::kScaleOffset) +
-                       (at % G::kScaleSlots) * 3 * kBN + tid;
+                       (at % G::kScaleSlots) * G::kScaleWords;
           // Keys past the length have no weight.
           const bool in = (s.t0 + i) * kBN + tid < s.seq.len;
-          const bool finite = sv <= 0x1p+127f;
+          const bool finite = sv <= kMaxScale;
           // A V scale that is not finite makes the score NaN: it reaches the rows that see the key
           // and adds nothing to the sums of the others.
-          out[0] = !in ? 0.f : finite ? sk * a.scale_log2 : __int_as_float(0x7fffffff);
-          sv = sv < kMinScale ? kMinScale : sv;
-          out[kBN] = !in ? -INFINITY : finite ? __log2f(sv) : 0.f;
-          out[2 * kBN] = in && finite ? 1.f / sv : 0.f;
+          out[tid] = !in ? 0.f : finite ? sk * a.scale_log2 : __int_as_float(0x7fffffff);
+          sv = fmaxf(sv, kMinScale);
+          const float log2_sv = !in ? -INFINITY : finite ? __log2f(sv) : 0.f;
+          out[kBN + tid] = log2_sv;
+          out[2 * kBN + tid] = in && finite ? 1.f / sv : 0.f;
+          care = care || __any_sync(0xffffffffu, in && !(log2_sv >= -40.f && log2_sv <= 45.f));
+          if ((tid & 31) == 0) reinterpret_cast<uint8_t*>(out + G::kCareAt)[tid >> 5] = care ? 1 : 0;
           mbar_arrive(&sh->scale_full[at % G::kScaleSlots]);
           sk = sk_next;
           sv = sv_next;
@@ -1039,8 +1084,8 @@ __global__ void __launch_bounds__(256, kBatch == 4 ? 4 : 2) extend_merge_kernel(
       if (ml[i].x != -INFINITY) {
         const float m_new = fmaxf(m, ml[i].x);
         const float keep = ex2(m - m_new), f = ex2(ml[i].x - m_new);
+        l = scale_sum(l, m - m_new) + scale_sum(ml[i].y, ml[i].x - m_new);
         m = m_new;
-        l = l * keep + ml[i].y * f;
         acc[0] = acc[0] * keep + o0[i].x * f;
         acc[1] = acc[1] * keep + o0[i].y * f;
         acc[2] = acc[2] * keep + o0[i].z * f;

@@ -21,8 +21,9 @@
 //  * V^T is the A operand of O^T = V^T P^T, by transposed 8 x 8 matrix loads of byte pairs: a
 //    register then holds columns d and d + 1 of two keys, M rows g and g + 8 of the fragment. P
 //    becomes the B operand by an 8 x 8 transpose in registers.
-//  * The scales act as in extend.cu: z = s mult + log2 sv, w = 2^(z - M) in fp16, the row sum takes
-//    w / sv.
+//  * The scales act as in extend.cu: z = s mult + log2 sv, w = 2^(z - M) in fp16. The row sum takes its
+//    terms 2^(z - log2 sv - M) by an exponential of their own: w / sv would lose keys whose sv is 2^100
+//    below the largest. (One row of 8 sequences of 16K-32K keys takes 83 us with either.)
 #include <algorithm>
 
 #include "extend_work.cuh"
@@ -42,7 +43,7 @@ struct FewGeometry {
   static constexpr int kTileBytes = kBN * D;             // K or V codes
   static constexpr int kStages = D == 128 ? 4 : 8;       // 128 KB of codes
   static constexpr int kScaleOffset = kStages * 2 * kTileBytes;
-  static constexpr int kScaleBytes = 3 * kBN * 4;        // sk, log2 sv and 1 / sv of one stage
+  static constexpr int kScaleBytes = 2 * kBN * 4;        // sk and log2 sv of one stage
   static constexpr int kRawTiles = 8;                    // scales as read: see the scale warp
   static constexpr int kRawOffset = kScaleOffset + kStages * kScaleBytes;
   static constexpr int kJoinOffset = kRawOffset + kRawTiles * 2 * kBN * 4;
@@ -72,11 +73,6 @@ __device__ __forceinline__ void cp_async_4(uint32_t dst, const float* src, bool 
 __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -239,7 +235,7 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
   }
   if (warp == G::kScaleWarp) {
     // ------------------------------- scales -------------------------------
-    // Lane i turns the scales of keys 4 i .. 4 i + 3 of a tile into sk, log2 sv and 1 / sv. They lie
+    // Lane i turns the scales of keys 4 i .. 4 i + 3 of a tile into sk and log2 sv. They lie
     // in one page, as 16 contiguous bytes with a.wide_scales. They are copied to shared memory
     // kRawTiles - 1 tiles ahead, each lane its own: a warp alone runs about 5 clocks per instruction
     // and cannot wait for memory in every tile (registers one tile ahead: 2200 clocks per
@@ -297,25 +293,26 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
         asm volatile("cp.async.wait_group %0;" ::"n"(kRawTiles - 1) : "memory");
         const float4* from = reinterpret_cast<const float4*>(
             smem + G::kRawOffset + (tile - s.t0) % kRawTiles * (2 * kBN * 4)) + lane;
-        const float4 sk = from[0];
+        const float4 sk4 = from[0];
         const float4 sv4 = from[kBN / 4];
+        float sk[4] = {sk4.x, sk4.y, sk4.z, sk4.w};
         const float sv[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
         const int st = issued % kStages;
         ok = issued < kStages || mbar_wait(&sh->empty[st], ((issued / kStages) - 1) & 1, guard);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        float add[4], inv[4];
+        float add[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float v = sv[i] < kMinScale ? kMinScale : sv[i];
-          add[i] = lg2(v);
-          // A scale that is not finite reaches the rows that see its key through z only.
-          inv[i] = v <= 0x1p+127f ? rcp(v) : 0.f;
+          // A V scale that is not finite makes the score NaN: it reaches the rows that see the key
+          // and adds nothing to the sums of the others.
+          const bool finite = sv[i] <= kMaxScale;
+          if (!finite) sk[i] = __int_as_float(0x7fffffff);
+          add[i] = finite ? lg2(fmaxf(sv[i], kMinScale)) : 0.f;
         }
         float4* dst = reinterpret_cast<float4*>(smem + G::kScaleOffset + st * G::kScaleBytes) + lane;
-        dst[0] = sk;
+        dst[0] = make_float4(sk[0], sk[1], sk[2], sk[3]);
         dst[kBN / 4] = make_float4(add[0], add[1], add[2], add[3]);
-        dst[2 * (kBN / 4)] = make_float4(inv[0], inv[1], inv[2], inv[3]);
         mbar_arrive(&sh->full[st]);
         ++issued;
       }
@@ -450,7 +447,6 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
       }
       const float sk[2] = {scales[0], scales[8]};
       const float add[2] = {scales[kBN], scales[kBN + 8]};
-      const float inv[2] = {scales[2 * kBN], scales[2 * kBN + 8]};
       // Element e: row e & 1, key g + 8 (e >> 1). The reference point moves only when a score
       // passes it by more than 2^8, and the warp's maximum is taken only then.
       bool above = false;
@@ -475,8 +471,8 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             if (mx > m_ref[nb][r] + kRescaleThreshold) {
               const float factor = ex2(m_ref[nb][r] - mx);   // 0 for the first keys
+              l_sum[nb][r] = scale_sum(l_sum[nb][r], m_ref[nb][r] - mx);
               m_ref[nb][r] = mx;
-              l_sum[nb][r] *= factor;
 #pragma unroll
               for (int c = 0; c < kSteps; ++c) {
                 o[nb][c][r] *= factor;
@@ -493,8 +489,11 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
         for (int e = 0; e < 4; ++e) {
           const int r = e & 1;
           const float ref = m_ref[nb][r] == -INFINITY ? 0.f : m_ref[nb][r];
-          z[nb][e] = ex2(z[nb][e] - ref);
-          l_sum[nb][r] = fmaf(z[nb][e], inv[e >> 1], l_sum[nb][r]);
+          const float x = z[nb][e] - ref;
+          z[nb][e] = ex2(x);
+          // The square of a root: the term may be below the exponential's range, 2^-126.
+          const float root = ex2(fmaf(x, 0.5f, -0.5f * add[e >> 1]));
+          l_sum[nb][r] = fmaf(root, root, l_sum[nb][r]);
         }
         pb[nb][0] = transpose8x8(pack2<__half>(z[nb][0], z[nb][1]));
         pb[nb][1] = transpose8x8(pack2<__half>(z[nb][2], z[nb][3]));
@@ -557,9 +556,9 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2(join_m[w * kRows + row] - top);
+        const float d = join_m[w * kRows + row] - top, f = ex2(d);
         const float4 x = *reinterpret_cast<const float4*>(join_o + (w * kRows + row) * D + col);
-        l = fmaf(join_l[w * kRows + row], f, l);
+        l += scale_sum(join_l[w * kRows + row], d);
         acc.x = fmaf(x.x, f, acc.x);
         acc.y = fmaf(x.y, f, acc.y);
         acc.z = fmaf(x.z, f, acc.z);

@@ -22,6 +22,7 @@ constexpr float kRescaleThreshold = 8.0f;   // log2 units: weights stay <= 2^8
 constexpr int kItemUnits = 2;         // fixed cost of an item, in halves of a two-tile key tile
 constexpr int kMaxBatch = 16384;      // the units' prefix sums use the K/V ring before it fills
 constexpr float kMinScale = 0x1p-100f;
+constexpr float kMaxScale = 0x1p+127f;   // V scales above it make the rows that see their key NaN
 constexpr int kMaxCtas = 256;         // SMs of a device (one CTA each)
 
 struct ExtendArgs {
@@ -185,6 +186,15 @@ struct Walk {
     return false;
   }
 };
+
+// l 2^d, d <= 0, for a row sum l. Over an int8 cache the sum is in units of 2^M where M holds the log2 of
+// a V scale, 2^-100 to 2^127: l can be 2^100 while M is far below the reference point it moves to, and
+// 2^d alone would be 0.
+__device__ __forceinline__ float scale_sum(float l, float d) {
+  if (d > -100.f) return l * ex2(d);
+  const float half = ex2(0.5f * d);
+  return (l * half) * half;
+}
 
 // x / y for 0 <= x, 0 < y: 32-bit where both fit (a 64-bit division takes hundreds of clocks).
 __device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {

@@ -6,8 +6,8 @@ A cache is [B, S_max, H_kv, D], or paged [num_blocks, page_size, H_kv, D] with b
 [B, max_blocks] int32, of the tokens' dtype or int8. An int8 cache holds one fp32 scale per token
 and KV head in k_scale / v_scale, [B, S_max, H_kv] or [num_blocks, page_size, H_kv] with any
 strides: the row x of one token and head is stored as round(x * 127 / max|x|) and max|x| / 127
-(2^-100 at least; the attention kernels read a smaller or negative v_scale as that). The attention
-kernels read scales along the keys of one head, so scales stored head by head
+(2^-100 at least; the attention kernels read a smaller or negative v_scale as that, and one above 2^127
+as NaN). The attention kernels read scales along the keys of one head, so scales stored head by head
 (`torch.empty(blocks, H_kv, page_size).transpose(1, 2)`) are read with wider loads.
 
 New rows are ragged: [T, H, D] with cu_seqlens [B + 1] int32, where sequence b owns rows

@@ -7,7 +7,7 @@ import torch
 
 import flash_lab
 from flash_lab import ops
-from test_kvcache import Cache, check_extend, check_rows
+from test_kvcache import Cache, check_extend, check_rows, host64
 
 BOTH = pytest.mark.parametrize("int8", [False, True], ids=["16bit", "int8"])
 DIMS = pytest.mark.parametrize("d", [64, 128])
@@ -56,3 +56,84 @@ def test_extend_left_padded_uniform_rows(d, int8):
         for b in range(96):
             k, v = cache.keys(b)
             check_rows(out[b], lse[b], q[b], k, v, True, d ** -0.5, int8)
+
+
+# ------------------------------------------------------------------------------------------------
+# V scales of an int8 cache
+# ------------------------------------------------------------------------------------------------
+
+def int8_cache_with_v_scales(lens, heads_kv, d, dtype, steps, zeros, **kw):
+    """An int8 cache whose V rows have the scales `steps` (float64 [sum(lens)]), and codes of 0 and the
+    smallest scale where `zeros`, as append_kv stores a row of zeros."""
+    cache = Cache(lens, heads_kv, d, dtype, True, **kw)
+    steps = np.where(zeros, 2.0 ** -100, steps).astype(np.float32)
+    full = torch.from_numpy(np.repeat(steps[:, None], heads_kv, 1)).cuda()
+    cache.put(cache.scales["v_scale"], full)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    codes = torch.randint(-127, 128, (sum(lens), heads_kv, d), device="cuda", generator=gen)
+    codes[torch.from_numpy(zeros).cuda()] = 0
+    cache.put(cache.v, codes.to(torch.int8))
+    cache.host["v"] = codes.double().cpu().numpy() * steps.astype(np.float64)[:, None, None]
+    return cache
+
+
+# Where the rows of zeros lie: a third of the keys at random, the first or the last of each sequence (other
+# key tiles, CTAs and warps than the rest), or all keys but one.
+PLACES = {
+    "mixed": lambda pos, n, rng: rng.rand(n) < 0.33,
+    "first": lambda pos, n, rng: pos < n // 2,
+    "last": lambda pos, n, rng: pos >= n // 2,
+    "all but one": lambda pos, n, rng: pos != n // 3,
+}
+
+
+@pytest.mark.gpu
+@DIMS
+@pytest.mark.parametrize("where", PLACES)
+@pytest.mark.parametrize("size", [2.0 ** 30, 2.0 ** 120, 2.0 ** -100], ids=["2^30", "2^120", "2^-100"])
+@pytest.mark.parametrize("new", [1, 40, 90], ids=lambda n: f"{n}rows")
+def test_extend_int8_rows_of_zeros_beside_large_ones(new, size, where, d):
+    """Rows of zeros count in the row sum however large the other rows of V are. One row runs in the
+    few-row kernel, 40 and 90 rows of 2 heads in items of one and of two tiles; a sequence has one to
+    eight key tiles, and 60 sequences put several of them into a CTA.
+
+    The bounds of check_rows hold: log2 of a scale r, |r| <= 127, enters an exponent and leaves it
+    again, three roundings at magnitudes up to 256 (2^-17 ln 2 each), and the reference point and the
+    logarithm of the sum are two more at up to 128 (2^-18 each), together less than 2.4e-5: S is 6
+    and more, so (d + 8) 2^-24 S + 2^-19 alone is 2.7e-5."""
+    rng = np.random.RandomState(11)
+    lens = [int(x) for x in rng.randint(new + 30, 300, 60)] + [1000]
+    steps = np.concatenate([size * 2.0 ** -rng.randint(0, 3, n).astype(np.float64) if size > 1 else
+                            np.full(n, size) for n in lens])
+    zeros = np.concatenate([PLACES[where](np.arange(n), n, rng) for n in lens])
+    cache = int8_cache_with_v_scales(lens, 2, d, torch.bfloat16, steps, zeros)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q = (3.0 * torch.randn(new * 61, 4, d, device="cuda", generator=gen)).bfloat16()
+    for b in range(61):
+        size = np.einsum("tgd,sd->tgs", np.abs(host64(q[b * new:b * new + new, :2])),
+                         np.abs(cache.keys(b)[0][:31, 0])) * d ** -0.5   # keys that every row sees
+        assert size.max(axis=-1).min() >= 6
+    check_extend(cache, [new] * 61, 4, torch.bfloat16, q=q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40], ids=["few", "many"])
+def test_extend_int8_v_scales_past_the_largest(new):
+    # A V scale above 2^127, an infinite one and a NaN one make the rows that see their key NaN, in both
+    # kernels; 2^127 itself is read.
+    for bad in (float("inf"), float("nan"), 1.5 * 2.0 ** 127):
+        cache = Cache([300], 1, 64, torch.bfloat16, True)
+        cache.scales["v_scale"][0, 290] = bad
+        q = torch.randn(new, 2, 64, device="cuda").bfloat16()
+        out, lse = flash_lab.extend(q, cache.k, cache.v, cache.seq_lens, torch.tensor(
+            [0, new], dtype=torch.int32, device="cuda"), return_lse=True, **cache.kwargs())
+        first = max(0, new - 10)   # row i sees keys up to 300 - new + i
+        assert torch.isnan(out[first:]).all() and torch.isnan(lse[first:]).all()
+        assert torch.isfinite(out[:first]).all() and torch.isfinite(lse[:first]).all()
+    zeros = np.zeros(300, dtype=bool)
+    steps = np.full(300, 2.0 ** 100)
+    steps[7] = 2.0 ** 127
+    cache = int8_cache_with_v_scales([300], 1, 64, torch.bfloat16, steps, zeros)
+    cache.v[0, 7] = (cache.v[0, 7] > 0).to(torch.int8)   # 2^127 or 0
+    cache.host["v"][7] = cache.v[0, 7].double().cpu().numpy() * 2.0 ** 127
+    check_extend(cache, [new], 2, torch.bfloat16)
