@@ -321,7 +321,9 @@ def _extend_checked(entry, q, k_cache, v_cache, seq_lens, cu_seqlens, block_tabl
     if q.dim() == 4:
         out, lse = out.view(q.shape), lse.view(q.shape[:3])
     if fast is not None:
-        fast.extend_known(entry, *args, ops._status_ptr(q.device), ops._sm_count(q.device))
+        status = ops._status_ptr(q.device)
+        if status:   # none: the first call of a device, under capture; recorded when it has one
+            fast.extend_known(entry, *args, status, ops._sm_count(q.device))
     return out, lse
 
 

@@ -513,12 +513,14 @@ def decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seq_le
         # Validation and the implementation choice depend only on what the key holds (shapes,
         # strides, dtypes, devices and the arguments), so later calls with the same key go
         # straight to the binding with the same arguments (a [B, 1, H, D] q is passed as is; the
-        # binding returns o in its shape).
-        if len(_DECODE_CALLS) >= 4096:
-            _DECODE_CALLS.clear()
-        _DECODE_CALLS[fast_key] = (float(scale), int(num_splits or 0),
-                                   spec.op != "decode_inplace", _status_ptr(q.device),
-                                   _sm_count(q.device))
+        # binding returns o in its shape). A device has no status word while its first call is being
+        # captured: such a call is not recorded.
+        status = _status_ptr(q.device)
+        if status:
+            if len(_DECODE_CALLS) >= 4096:
+                _DECODE_CALLS.clear()
+            _DECODE_CALLS[fast_key] = (float(scale), int(num_splits or 0),
+                                       spec.op != "decode_inplace", status, _sm_count(q.device))
     if block_tables is None:
         out, lse = _call_op(spec.op, q3, k_cache, v_cache, seq_lens, scale, num_splits or 0)
     else:

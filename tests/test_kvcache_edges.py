@@ -137,3 +137,46 @@ def test_extend_int8_v_scales_past_the_largest(new):
     cache.v[0, 7] = (cache.v[0, 7] > 0).to(torch.int8)   # 2^127 or 0
     cache.host["v"][7] = cache.v[0, 7].double().cpu().numpy() * 2.0 ** 127
     check_extend(cache, [new], 2, torch.bfloat16)
+
+
+# ------------------------------------------------------------------------------------------------
+# Records of checked calls
+# ------------------------------------------------------------------------------------------------
+
+class FakeBinding:
+    """The binding's records, without kernels."""
+
+    def __init__(self):
+        self.known = []
+
+    def extend_fast(self, *args):
+        return None
+
+    def extend_known(self, *args):
+        self.known.append(args)
+
+    def decode(self, *args):
+        raise AssertionError("a recorded call ran")
+
+
+def test_calls_without_a_status_word_are_not_recorded(monkeypatch):
+    # While a graph is captured, a device that has no status word yet gets none: a call recorded then would
+    # run without one for good, and its timed-out waits would never be reported.
+    q = torch.zeros(2, 4, 64, dtype=torch.float16)
+    kc, vc = (torch.zeros(2, 16, 2, 64, dtype=torch.float16) for _ in range(2))
+    lens = torch.full((2,), 16, dtype=torch.int32)
+    status = 0
+    binding = FakeBinding()
+    monkeypatch.setattr(ops, "_NATIVE", binding)
+    monkeypatch.setattr(ops, "DEBUG", False)
+    monkeypatch.setattr(ops, "_DECODE_CALLS", {})
+    monkeypatch.setattr(ops, "_status_ptr", lambda device: status)
+    monkeypatch.setattr(ops, "_sm_count", lambda device: 148)
+    monkeypatch.setattr(ops, "_select_cached", lambda *args: ops.DECODE_IMPLS["splitkv"])
+    monkeypatch.setattr(ops, "_call_op", lambda name, q, *args: (q, q[..., 0].float()))
+    monkeypatch.setattr("flash_lab.kvcache._require_kernels", lambda device: None)
+    for status, records in ((0, 0), (4096, 1)):
+        flash_lab.extend(q, kc, vc, lens)
+        flash_lab.decode(q, kc, vc, lens)
+        assert len(binding.known) == len(ops._DECODE_CALLS) == records
+    assert binding.known[0][-2] == 4096 and next(iter(ops._DECODE_CALLS.values()))[3] == 4096
