@@ -65,7 +65,7 @@ struct Ragged {
 };
 
 // Where row t of a ragged call lives: the sequence b that owns it, its place in the sequence and
-// the sequence's row count; false if no sequence owns it. Lane i of a warp asks for row t0 + i.
+// the sequence's row count, of the rows that there are; false if no sequence owns it. Lane i of a warp asks for row t0 + i.
 // cu is searched 32 ways at once for t0 (one dependent load per factor of 32 of the batch), and
 // from there each lane steps to its own row's sequence.
 __device__ __forceinline__ bool find_sequences(const Ragged& r, int t0, int lane, int& b, int& place,
@@ -73,8 +73,9 @@ __device__ __forceinline__ bool find_sequences(const Ragged& r, int t0, int lane
   const int t = t0 + lane;
   if (r.cu == nullptr) {
     b = t / r.rows_per_seq;
-    place = t - b * r.rows_per_seq;
-    count = r.rows_per_seq;
+    const int start = b * r.rows_per_seq;   // at most t
+    place = t - start;
+    count = min(r.rows_per_seq, r.rows - start);
     return t < r.rows && b < r.batch;
   }
   int lo = 0, hi = r.batch;   // the largest b in [lo, hi) with cu[b] <= t0, or 0
@@ -94,9 +95,11 @@ __device__ __forceinline__ bool find_sequences(const Ragged& r, int t0, int lane
     first = end;
     end = __ldg(r.cu + b + 1);
   }
+  first = max(first, 0);
+  end = min(end, r.rows);
   place = t - first;
   count = end - first;
-  return t < r.rows && first <= t && t < end;
+  return first <= t && t < end;
 }
 
 // Checks of an flb_kv_cache that do not depend on who uses it: required pointers, positive sizes,

@@ -1,13 +1,15 @@
 """More of the KV-cache operators at their edges: batches padded on the left, and what the other tests
 of test_kvcache.py, whose helpers and tolerances these use, do not reach."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import flash_lab
-from flash_lab import ops
-from test_kvcache import Cache, check_extend, check_rows, host64
+from flash_lab import _capi, ops
+from test_kvcache import Cache, check_extend, check_rows, host64, offsets
 
 BOTH = pytest.mark.parametrize("int8", [False, True], ids=["16bit", "int8"])
 DIMS = pytest.mark.parametrize("d", [64, 128])
@@ -180,3 +182,57 @@ def test_calls_without_a_status_word_are_not_recorded(monkeypatch):
         flash_lab.decode(q, kc, vc, lens)
         assert len(binding.known) == len(ops._DECODE_CALLS) == records
     assert binding.known[0][-2] == 4096 and next(iter(ops._DECODE_CALLS.values()))[3] == 4096
+
+
+# ------------------------------------------------------------------------------------------------
+# Offsets past the rows
+# ------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@BOTH
+def test_append_and_extend_agree_on_offsets_past_the_rows(int8):
+    # Offsets are clamped to the rows that there are: of 10 and 3 promised rows the second sequence has
+    # one, and they are its last keys for append_kv as for extend.
+    lens, cu = [12, 9], torch.tensor([-4, 10, 13], dtype=torch.int32, device="cuda")
+    cache = Cache(lens, 2, 64, torch.float16, int8, page=8)
+    k, v = (torch.randn(11, 2, 64, device="cuda").half() for _ in range(2))
+    flash_lab.append_kv(k, v, cache.k, cache.v, cache.seq_lens, cu, **cache.kwargs())
+    got = flash_lab.gather_kv(cache.k, cache.v, cache.seq_lens, offsets(lens), 21,
+                              dtype=torch.float32 if int8 else None, **cache.kwargs())
+    for x, y, name in zip(got, (k, v), "kv"):
+        want = torch.from_numpy(cache.host[name]).cuda()
+        want[2:12], want[20] = y[:10].double(), y[10].double()
+        # int8 rows: half a step and a few fp32 roundings; values as they are otherwise.
+        step = want.abs().amax(-1, keepdim=True) / 127 if int8 else 0.0
+        assert ((x.double() - want).abs() <= 0.501 * step).all()
+        cache.host[name] = host64(x)
+    q = torch.randn(11, 4, 64, device="cuda").half()
+    out, lse = flash_lab.extend(q, cache.k, cache.v, cache.seq_lens, cu, return_lse=True,
+                                **cache.kwargs())
+    check_rows(out[:10], lse[:10], q[:10], *cache.keys(0), True, 0.125, int8)
+    check_rows(out[10:], lse[10:], q[10:], *cache.keys(1), True, 0.125, int8)
+
+
+@pytest.mark.gpu
+def test_append_of_fewer_rows_than_the_sequences_have():
+    # rows < batch * rows_per_seq (C entry only): the last sequence has what is left, one row.
+    lib = _capi.load()
+    cache = Cache([6, 6], 1, 64, torch.float16, poison=False)
+    before = cache.k.clone(), cache.v.clone()
+    k = torch.randn(4, 1, 64, device="cuda").half()
+    c = cache_struct(cache)
+    r = _capi.KVRows(k.data_ptr(), k.data_ptr(), 64, 64, 64, 64, 0, cache.seq_lens.data_ptr(), 4, 3,
+                     _capi.FLB_FP16)
+    assert lib.flb_kv_append(ctypes.byref(c), ctypes.byref(r),
+                             torch.cuda.current_stream().cuda_stream) == 0
+    for x, y in zip((cache.k, cache.v), before):
+        y[0, 3:6], y[1, 5] = k[:3], k[3]
+        assert torch.equal(x, y)
+
+
+def cache_struct(cache):
+    """The C entries' view of a Cache."""
+    from flash_lab import kvcache
+
+    return kvcache._cache_struct(cache.k, cache.v, cache.seq_lens, cache.block_tables,
+                                 cache.scales.get("k_scale"), cache.scales.get("v_scale"))
