@@ -236,3 +236,78 @@ def cache_struct(cache):
 
     return kvcache._cache_struct(cache.k, cache.v, cache.seq_lens, cache.block_tables,
                                  cache.scales.get("k_scale"), cache.scales.get("v_scale"))
+
+
+# ------------------------------------------------------------------------------------------------
+# Nothing outside the buffers
+# ------------------------------------------------------------------------------------------------
+
+class Guarded:
+    """Tensors inside larger ones whose other bytes must stay as they were."""
+
+    def __init__(self):
+        self.all = []
+
+    def __call__(self, *shape, dtype, like=None):
+        n = int(np.prod(shape))
+        pad = 4096
+        big = torch.full((n + 2 * pad,), 77, dtype=dtype, device="cuda")
+        inside = big[pad:pad + n].view(shape)
+        if like is not None:
+            inside.copy_(like)
+        self.all.append((big, pad, n))
+        return inside
+
+    def intact(self):
+        return all((big[:pad] == 77).all() and (big[pad + n:] == 77).all()
+                   for big, pad, n in self.all)
+
+
+@pytest.mark.gpu
+@BOTH
+@pytest.mark.parametrize("cu", [[0, 64, 0, 64], [64, 0, 64, 0], [10 ** 9, -5, 10 ** 9, 3], [5, 5, 5, 5],
+                                [-(2 ** 31), 2 ** 31 - 1, -1, 70], [0, 2, 4, 6]],
+                         ids=lambda cu: "_".join(map(str, cu)))
+def test_offsets_of_any_kind_write_only_the_outputs(cu, int8):
+    """Offsets that decrease or run past the rows are no valid calls, and their rows are unspecified: the
+    calls end, and nothing outside the outputs and the cache is written."""
+    lib = _capi.load()
+    rows, heads, heads_kv, d = 64, 8, 2, 64
+    guard = Guarded()
+    cache = Cache([300, 200, 100], heads_kv, d, torch.bfloat16, int8, page=16, poison=False)
+    cache.k, cache.v = (guard(*x.shape, dtype=x.dtype, like=x) for x in (cache.k, cache.v))
+    for name, x in cache.scales.items():
+        cache.scales[name] = guard(*x.shape, dtype=torch.float32, like=x)
+    kept = [x.clone() for x in (cache.k, cache.v, *cache.scales.values())]
+    cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    q = torch.randn(rows, heads, d, device="cuda").bfloat16()
+    o = guard(rows, heads, d, dtype=torch.bfloat16)
+    lse = guard(rows, heads, dtype=torch.float32)
+    need = lib.flb_extend_workspace_bytes(rows, heads, heads_kv, d, ops._sm_count(q.device))
+    ws = guard(need, dtype=torch.uint8)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    c = cache_struct(cache)
+    p = _capi.ExtendParams(q.data_ptr(), o.data_ptr(), lse.data_ptr(), q.stride(0), q.stride(1),
+                           o.stride(0), o.stride(1), cu.data_ptr(), cache.seq_lens.data_ptr(), rows, 0,
+                           heads, 1, _capi.FLB_BF16, 0.125, ws.data_ptr(), need, status.data_ptr())
+    assert lib.flb_extend_fwd(ctypes.byref(c), ctypes.byref(p), stream) == 0
+    gathered = [guard(rows, heads_kv, d, dtype=torch.bfloat16) for _ in range(2)]
+    r = _capi.KVRows(gathered[0].data_ptr(), gathered[1].data_ptr(), heads_kv * d, d, heads_kv * d, d,
+                     cu.data_ptr(), cache.seq_lens.data_ptr(), rows, 0, _capi.FLB_BF16)
+    assert lib.flb_kv_gather(ctypes.byref(c), ctypes.byref(r), stream) == 0
+    torch.cuda.synchronize()
+    assert int(status) == 0 and guard.intact()
+    assert all(torch.equal(a, b) for a, b in zip(kept, (cache.k, cache.v, *cache.scales.values())))
+    new = [torch.randn(rows, heads_kv, d, device="cuda").bfloat16() for _ in range(2)]
+    r = _capi.KVRows(new[0].data_ptr(), new[1].data_ptr(), heads_kv * d, d, heads_kv * d, d,
+                     cu.data_ptr(), cache.seq_lens.data_ptr(), rows, 0, _capi.FLB_BF16)
+    assert lib.flb_kv_append(ctypes.byref(c), ctypes.byref(r), stream) == 0
+    torch.cuda.synchronize()
+    assert guard.intact()
+    # Pages of no sequence are as they were, too.
+    used = cache.block_tables[cache.block_tables < cache.outer].long().unique()
+    other = torch.ones(cache.outer, dtype=torch.bool, device="cuda")
+    other[used] = False
+    for now, then in zip((cache.k, cache.v, *cache.scales.values()), kept):
+        assert torch.equal(now[other], then[other])
