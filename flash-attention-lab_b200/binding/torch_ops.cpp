@@ -298,16 +298,20 @@ std::tuple<at::Tensor, at::Tensor> kv_gather(const at::Tensor& k_cache, const at
   return {k, v};
 }
 
-std::tuple<at::Tensor, at::Tensor> extend(const at::Tensor& q, const at::Tensor& k_cache,
+std::tuple<at::Tensor, at::Tensor> extend(const at::Tensor& q_in, const at::Tensor& k_cache,
                                           const at::Tensor& v_cache, const at::Tensor& seq_lens,
                                           const OptTensor& cu_seqlens,
                                           const OptTensor& block_tables, const OptTensor& k_scale,
                                           const OptTensor& v_scale, int64_t rows_per_seq,
                                           bool causal, double scale, int64_t status,
                                           int64_t sm_count) {
-  if (q.dim() != 3 || q.stride(2) != 1)
+  if (q_in.dim() != 3 || q_in.stride(2) != 1)
     throw std::runtime_error("q must be [rows, H, D], contiguous in head_dim");
-  const c10::cuda::CUDAGuard guard(q.device());
+  const c10::cuda::CUDAGuard guard(q_in.device());
+  // Queries expanded over rows or heads are copied.
+  const bool expanded = (q_in.size(0) > 1 && q_in.stride(0) == 0) ||
+                        (q_in.size(1) > 1 && q_in.stride(1) == 0);
+  const at::Tensor q = expanded ? q_in.contiguous() : q_in;
   const flb_kv_cache c = cache_struct(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale);
   if (q.size(2) != c.head_dim) throw std::runtime_error("q and the cache differ in head_dim");
   if (cu_seqlens.has_value() && cu_seqlens->numel() != int64_t{c.batch} + 1)

@@ -513,8 +513,10 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
         const TmaCoords& c = is_v ? a.vc : a.kc;
         const int key = tile * kBN + part * a.box_rows;
         const int row = paged ? key - a.cache.page.div(key) * a.cache.page.d : key;
-        tma_load_4d(dst, is_v ? &tmv : &tmk, full, col * 64, tma_c(c, 1, row, s.hkv, blk),
-                    tma_c(c, 2, row, s.hkv, blk), tma_c(c, 3, row, s.hkv, blk));
+        const int once = is_v ? a.v_once : a.k_once;
+        const int h = coordinate(s.hkv, once & kOnceHeads), at = coordinate(blk, once & kOnceOuter);
+        tma_load_4d(dst, is_v ? &tmv : &tmk, full, col * 64, tma_c(c, 1, row, h, at),
+                    tma_c(c, 2, row, h, at), tma_c(c, 3, row, h, at));
       }
       ++(is_v ? v_issued : k_issued);
       return true;
@@ -1207,6 +1209,12 @@ int validate(const flb_kv_cache* c, const flb_extend_params* p) {
                 c->dtype);
   if (!(p->softmax_scale > 0.f) || !(p->softmax_scale <= 3.0e38f))
     return fail(FLB_ERR_INVALID_ARGUMENT, "softmax_scale must be positive and finite");
+  const int cache_rows = c->block_tables != nullptr ? c->page_size : c->max_seqlen;
+  if ((p->rows > 1 && (p->q_row_stride == 0 || p->o_row_stride == 0)) ||
+      (p->heads > 1 && (p->q_head_stride == 0 || p->o_head_stride == 0)) ||
+      (cache_rows > 1 && (c->k_seq_stride == 0 || c->v_seq_stride == 0)))
+    return fail(FLB_ERR_UNSUPPORTED,
+                "rows and heads of q and o, and keys, must lie apart: found a stride 0");
   const int ps = c->page_size;
   if (c->block_tables != nullptr && !(ps == 8 || ps == 16 || ps == 32 || ps % 64 == 0))
     return fail(FLB_ERR_UNSUPPORTED, "paged cache: page_size %d must be 8, 16, 32 or a multiple of 64",
@@ -1337,7 +1345,9 @@ extern "C" int flb_extend_fwd(const flb_kv_cache* c, const flb_extend_params* p,
   set_partials(&a, ws + partial_bytes(sm_count, kFewTile, c->head_dim), sm_count,
                part_rows(p->rows, a.group));
   CUtensorMap tmq, tmk, tmv;
-  const View4 kv = kv_view4(c, false), vv = kv_view4(c, true);
+  View4 kv = kv_view4(c, false), vv = kv_view4(c, true);
+  a.k_once = fold_expanded(&kv);
+  a.v_once = fold_expanded(&vv);
   if (int8) {
     if (int st = encode_rows_map(&tmk, &a.kc, kv, a.box_rows, c->head_dim, FLB_INT8, 0)) return st;
     if (int st = encode_rows_map(&tmv, &a.vc, vv, a.box_rows, c->head_dim, FLB_INT8, 0)) return st;

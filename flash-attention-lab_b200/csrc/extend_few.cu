@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
     const bool paged = a.cache.block_tables != nullptr;
     const CUtensorMap* map = is_v ? &tmv : &tmk;
     const TmaCoords& c = is_v ? a.vc : a.kc;
+    const int once = is_v ? a.v_once : a.k_once;
     BlockWindow window;
     int issued = 0;
     bool ok = true;
@@ -220,10 +221,12 @@ __global__ void __launch_bounds__(FewGeometry<D, kBlocks>::kThreads, 1)
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&sh->full[st], G::kTileBytes);
         __syncwarp();
-        if (issues)
+        if (issues) {
+          const int h = coordinate(s.hkv, once & kOnceHeads), at = coordinate(blk, once & kOnceOuter);
           tma_load_4d(smem + (2 * st + (is_v ? 1 : 0)) * G::kTileBytes + offset * D, map,
-                      &sh->full[st], 0, tma_c(c, 1, row, s.hkv, blk), tma_c(c, 2, row, s.hkv, blk),
-                      tma_c(c, 3, row, s.hkv, blk));
+                      &sh->full[st], 0, tma_c(c, 1, row, h, at), tma_c(c, 2, row, h, at),
+                      tma_c(c, 3, row, h, at));
+        }
         ++issued;
       }
     }
@@ -642,10 +645,11 @@ int launch_extend_few(const ExtendArgs& args, const flb_kv_cache* c, const void*
   const QueryView qv{q, {q_row_stride, q_head_stride}};
   CUtensorMap tmk, tmv;
   const int d = c->head_dim;
-  if (int st = encode_rows_map(&tmk, &a.kc, kv_view4(c, false), a.box_rows, d, FLB_INT8, d))
-    return st;
-  if (int st = encode_rows_map(&tmv, &a.vc, kv_view4(c, true), a.box_rows, d, FLB_INT8, d))
-    return st;
+  View4 kv = kv_view4(c, false), vv = kv_view4(c, true);
+  a.k_once = fold_expanded(&kv);
+  a.v_once = fold_expanded(&vv);
+  if (int st = encode_rows_map(&tmk, &a.kc, kv, a.box_rows, d, FLB_INT8, d)) return st;
+  if (int st = encode_rows_map(&tmv, &a.vc, vv, a.box_rows, d, FLB_INT8, d)) return st;
   const int rows = a.tile_tokens * a.group;   // the most score rows of a sequence
   if (dtype == FLB_BF16)
     return launch_t<__nv_bfloat16>(a, qv, tmk, tmv, d, rows, ctas, dev, stream);

@@ -41,6 +41,7 @@ struct ExtendArgs {
   int box_rows;                       // cache rows per TMA box (a box never crosses a page)
   float scale_log2;
   TmaCoords kc, vc;
+  int k_once, v_once;                 // expanded dimensions of K and V (fold_expanded)
   // Partials: slot 2 c + i is CTA c's first (0) or last (1) item share. part_o holds
   // [slots][D / 8][part_rows][8], part_ml [slots][part_rows][2].
   int part_rows;
@@ -60,6 +61,23 @@ enum : int { kPartValid = 1, kPartOpens = 2, kPartCloses = 4 };
 __device__ __forceinline__ int tma_c(const TmaCoords& c, int slot, int s, int h, int b) {
   return c.pos_s == slot ? s : (c.pos_h == slot ? h : b);
 }
+
+// Caches may be expanded over sequences (or blocks) and KV heads: such a dimension of stride 0 has size 1
+// in the tensor map, and its coordinate is 0 (or negative still: zeros).
+enum : int { kOnceOuter = 1, kOnceHeads = 2 };
+inline int fold_expanded(View4* v) {
+  int once = 0;
+  if (v->size[0] > 1 && v->stride[0] == 0) {
+    v->size[0] = 1;
+    once |= kOnceOuter;
+  }
+  if (v->size[2] > 1 && v->stride[2] == 0) {
+    v->size[2] = 1;
+    once |= kOnceHeads;
+  }
+  return once;
+}
+__device__ __forceinline__ int coordinate(int x, int once) { return once ? min(x, 0) : x; }
 
 // --------------------------------------------------------------------------------------------
 // The work

@@ -52,6 +52,11 @@ def _ptr(x) -> int:
     return 0 if x is None else x.data_ptr()
 
 
+def _expanded(x, dims) -> bool:
+    """Whether a dimension of x, among dims, repeats the same memory."""
+    return any(x.shape[i] > 1 and x.stride(i) == 0 for i in dims)
+
+
 def _cache_struct(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale):
     paged = block_tables is not None
     return _capi.KVCache(
@@ -116,6 +121,8 @@ def _extend(q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scale, v_
         if ops.DEBUG:
             ops._check(_capi.FLB_OK, "flb_extend_fwd", q.device)
         return o, lse
+    if _expanded(q, (0, 1)):
+        q = q.contiguous()
     rows, heads, head_dim = q.shape
     o = torch.empty((rows, heads, head_dim), dtype=q.dtype, device=q.device)
     lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device)
@@ -198,7 +205,7 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
                                cu_seqlens, {"k": k, "v": v})
     for name, x in (("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale),
                     ("v_scale", v_scale)):
-        if x is not None and any(n > 1 and st == 0 for n, st in zip(x.shape, x.stride())):
+        if x is not None and _expanded(x, range(x.dim())):
             raise ValueError(f"{name} is written and must not be expanded, got strides "
                              f"{tuple(x.stride())} for shape {tuple(x.shape)}")
     if k.shape != v.shape:
@@ -269,7 +276,8 @@ def extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seq_le
     cache has q's dtype or is int8 with k_scale and v_scale. With n new rows, row i of sequence b sees
     keys 0 .. seq_lens[b] - n + i (all seq_lens[b] keys when causal is False). seq_lens values are
     clamped to [0, S_max] on the device. Paged caches take pages of 8, 16, 32 or a multiple of 64
-    rows.
+    rows. Caches may be expanded over sequences or KV heads (a prefix that all sequences share);
+    a q expanded over rows or heads is copied.
 
     Returns o in q's shape and dtype and, with return_lse=True, the natural-log log-sum-exp of
     each score row as fp32 in q's shape without its last dimension. Rows that see no key, or
@@ -312,6 +320,8 @@ def _extend_checked(entry, q, k_cache, v_cache, seq_lens, cu_seqlens, block_tabl
                          f"{q3.shape[1]} and {shape.heads_kv}")
     if shape.page_size and not (shape.page_size in (8, 16, 32) or shape.page_size % 64 == 0):
         raise ValueError(f"page_size {shape.page_size} is not 8, 16, 32 or a multiple of 64")
+    if _expanded(k_cache, (1,)) or _expanded(v_cache, (1,)):
+        raise ValueError("caches must not be expanded along their keys")
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"softmax_scale must be positive, got {scale}")
     _check_head_dim(shape.head_dim)

@@ -341,7 +341,8 @@ int flb_kv_gather(const flb_kv_cache* cache, const flb_kv_rows* rows, flb_stream
  * causal is 1, all L keys otherwise. Rows that see no key or belong to no sequence give 0 and
  * an LSE of -inf. head_dim 64 or 128, H / H_kv at most 128, at most 16384 sequences, pages of 8, 16,
  * 32 or a multiple of 64 rows; pointers and strides of q, o and the caches are multiples of 16
- * bytes.
+ * bytes. A stride 0 over sequences or blocks, or over KV heads, repeats the cache's memory; rows and heads
+ * of q and o and the keys of a sequence lie apart.
  * workspace holds flb_extend_workspace_bytes(...) bytes; nothing in it needs initialising.
  */
 typedef struct {

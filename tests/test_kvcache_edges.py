@@ -9,7 +9,7 @@ import torch
 
 import flash_lab
 from flash_lab import _capi, ops
-from test_kvcache import Cache, check_extend, check_rows, host64, offsets
+from test_kvcache import Cache, _host_cache, check_extend, check_rows, host64, offsets
 
 BOTH = pytest.mark.parametrize("int8", [False, True], ids=["16bit", "int8"])
 DIMS = pytest.mark.parametrize("d", [64, 128])
@@ -311,3 +311,94 @@ def test_offsets_of_any_kind_write_only_the_outputs(cu, int8):
     other[used] = False
     for now, then in zip((cache.k, cache.v, *cache.scales.values()), kept):
         assert torch.equal(now[other], then[other])
+
+
+# ------------------------------------------------------------------------------------------------
+# Orders of strides
+# ------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@BOTH
+@DIMS
+@pytest.mark.parametrize("new", [(2, 1), (60, 40)], ids=["few", "many"])
+def test_extend_of_head_major_queries(new, d, int8):
+    # q as [H, T, D] seen through a transpose.
+    cache = Cache([150, 90], 2, d, torch.bfloat16, int8, head_major=True)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q = torch.randn(8, sum(new), d, device="cuda", generator=gen).bfloat16().transpose(0, 1)
+    check_extend(cache, list(new), 8, torch.bfloat16, q=q)
+
+
+@pytest.mark.gpu
+@BOTH
+def test_extend_of_strided_batches(int8):
+    # [B, n, H, D] whose sequences lie apart, and head-major ones that cannot be flattened in place.
+    cache = Cache([80, 33, 200], 2, 64, torch.float16, int8, page=8)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    base = torch.randn(3, 9, 4, 64, device="cuda", generator=gen).half()
+    for q in (base[:, 2:7], base.transpose(1, 2).contiguous().transpose(1, 2)[:, :5]):
+        for _ in range(2):   # checked, then recorded
+            out, lse = flash_lab.extend(q, cache.k, cache.v, cache.seq_lens, return_lse=True,
+                                        **cache.kwargs())
+            assert out.shape == q.shape and lse.shape == (3, 5, 4)
+            for b in range(3):
+                check_rows(out[b], lse[b], q[b], *cache.keys(b), True, 0.125, int8)
+
+
+@pytest.mark.gpu
+@BOTH
+@DIMS
+@pytest.mark.parametrize("new", [1, 40], ids=["few", "many"])
+def test_extend_of_expanded_tensors(new, d, int8):
+    # One prefix for all sequences, one KV head for several, and queries repeated over heads or tokens:
+    # the bits of the copied tensors.
+    cache = Cache([200, 200, 200], 4, d, torch.bfloat16, int8, capacity=210)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    q = torch.randn(3 * new, 8, d, device="cuda", generator=gen).bfloat16()
+    cu = offsets([new] * 3)
+
+    def run(q, k, v, scales):
+        for _ in range(2):   # checked, then recorded
+            got = flash_lab.extend(q, k, v, cache.seq_lens, cu, return_lse=True, **scales)
+        return got
+
+    def same(q, views):
+        copies = {name: x.contiguous() for name, x in views.items()}
+        got, want = (run(x, y.pop("k"), y.pop("v"), y)
+                     for x, y in ((q, dict(views)), (q.contiguous(), copies)))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert not torch.isnan(got[0]).any()
+
+    tensors = {"k": cache.k, "v": cache.v, **cache.scales}
+    same(q, {name: x[1:2].expand_as(x) for name, x in tensors.items()})
+    same(q, {name: x[:, :, 2:3].expand_as(x) for name, x in tensors.items()})
+    same(q, {**tensors, "v": cache.v[:1, :, :1].expand_as(cache.v)})
+    same(q[:, :1].expand_as(q), tensors)
+    same(q[:1].expand_as(q), tensors)
+
+
+def test_extend_refuses_overlapping_rows():
+    # C entry: queries and outputs are matrices of distinct rows, keys lie apart.
+    lib = _capi.load()
+    good = dict(q=1 << 20, o=1 << 20, lse=1 << 20, q_row_stride=1024, q_head_stride=128,
+                o_row_stride=1024, o_head_stride=128, cu_seqlens=1 << 20, seq_lens=1 << 20, rows=4,
+                heads=8, dtype=_capi.FLB_BF16, softmax_scale=0.1)
+    for changes in (dict(q_row_stride=0), dict(q_head_stride=0), dict(o_row_stride=0),
+                    dict(o_head_stride=0)):
+        p = _capi.ExtendParams(**{**good, **changes})
+        assert lib.flb_extend_fwd(ctypes.byref(_host_cache()), ctypes.byref(p), None) \
+            == _capi.FLB_ERR_UNSUPPORTED, changes
+        assert b"stride 0" in lib.flb_last_error()
+    for changes in (dict(k_seq_stride=0), dict(v_seq_stride=0)):
+        p = _capi.ExtendParams(**good)
+        assert lib.flb_extend_fwd(ctypes.byref(_host_cache(**changes)), ctypes.byref(p), None) \
+            == _capi.FLB_ERR_UNSUPPORTED, changes
+        assert b"stride 0" in lib.flb_last_error()
+
+
+def test_extend_refuses_caches_expanded_along_their_keys():
+    kc, vc = (torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16) for _ in range(2))
+    q, lens = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.full((2,), 16, dtype=torch.int32)
+    for k, v in ((kc[:, :1].expand_as(kc), vc), (kc, vc[:, :1].expand_as(vc))):
+        with pytest.raises(ValueError, match="along their keys"):
+            flash_lab.extend(q, k, v, lens)
