@@ -280,6 +280,15 @@ void kv_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cac
   const flb_kv_cache c = cache_struct(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale);
   const flb_kv_rows r = rows_struct(k, v, c, cu_seqlens, seq_lens, rows_per_seq);
   if (int st = flb_kv_append(&c, &r, current_stream(k))) raise_status("flb_kv_append", st);
+  // As for any in-place write, so that autograd notices where it had saved one of these. Tensors of
+  // inference mode have no version.
+  auto written = [](const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  written(k_cache);
+  written(v_cache);
+  if (k_scale.has_value()) written(*k_scale);
+  if (v_scale.has_value()) written(*v_scale);
 }
 
 std::tuple<at::Tensor, at::Tensor> kv_gather(const at::Tensor& k_cache, const at::Tensor& v_cache,

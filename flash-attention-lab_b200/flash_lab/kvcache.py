@@ -90,6 +90,9 @@ def _append(k, v, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scale,
             status = lib.flb_kv_append(ctypes.byref(cache), ctypes.byref(rows),
                                        ops._raw_stream(k.device))
         ops._check(status, "flb_kv_append", k.device)
+        for x in (k_cache, v_cache, k_scale, v_scale):
+            if x is not None and not x.is_inference():
+                torch.autograd.graph.increment_version(x)
 
 
 def _gather(k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scale, v_scale, total: int,

@@ -402,3 +402,40 @@ def test_extend_refuses_caches_expanded_along_their_keys():
     for k, v in ((kc[:, :1].expand_as(kc), vc), (kc, vc[:, :1].expand_as(vc))):
         with pytest.raises(ValueError, match="along their keys"):
             flash_lab.extend(q, k, v, lens)
+
+
+# ------------------------------------------------------------------------------------------------
+# In-place writes and arguments
+# ------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@BOTH
+def test_append_raises_version_counters(int8, monkeypatch):
+    # As any in-place write.
+    cache = Cache([5, 9], 2, 64, torch.bfloat16, int8, poison=False)
+    k = torch.randn(2, 2, 64, device="cuda").bfloat16()
+    written = [cache.k, cache.v, *cache.scales.values()]
+    for binding in (True, True, False):   # checked, recorded, without the binding
+        if not binding:
+            monkeypatch.setattr(ops, "_NATIVE", None)
+        before = [x._version for x in written]
+        flash_lab.append_kv(k, k, cache.k, cache.v, cache.seq_lens, **cache.kwargs())
+        assert all(x._version > v for x, v in zip(written, before))
+    monkeypatch.undo()
+    # Tensors of inference mode have no counter.
+    with torch.inference_mode():
+        other = Cache([5, 9], 2, 64, torch.bfloat16, int8, poison=False)
+        flash_lab.append_kv(k, k, other.k, other.v, other.seq_lens, **other.kwargs())
+    flash_lab.append_kv(k, k, other.k, other.v, other.seq_lens, **other.kwargs())
+    assert torch.equal(other.k, cache.k)
+
+
+@pytest.mark.gpu
+def test_autograd_notices_an_append():
+    cache = Cache([5, 9], 2, 64, torch.float32, poison=False)
+    k = torch.randn(2, 2, 64, device="cuda")
+    w = torch.ones_like(cache.k, requires_grad=True)
+    y = (w * cache.k).sum()   # saves the cache
+    flash_lab.append_kv(k, k, cache.k, cache.v, cache.seq_lens)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
