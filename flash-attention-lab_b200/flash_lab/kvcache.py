@@ -251,6 +251,8 @@ def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, seq_lens: torch.Tens
     shape = check_cache_inputs(k_cache, v_cache, seq_lens, block_tables, k_scale, v_scale, cu_seqlens)
     if cu_seqlens is None:
         raise TypeError("cu_seqlens must be a torch.Tensor, got NoneType")
+    if not hasattr(type(total), "__index__"):
+        raise TypeError(f"total must be an int, got {type(total).__name__}")
     if total < 1:
         raise ValueError(f"total must be positive, got {total}")
     out = dtype if dtype is not None else torch.bfloat16 if shape.int8 else k_cache.dtype

@@ -439,3 +439,31 @@ def test_autograd_notices_an_append():
     flash_lab.append_kv(k, k, cache.k, cache.v, cache.seq_lens)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_gather_total_is_an_integer():
+    kc = torch.zeros(2, 16, 2, 64)
+    lens, cu = torch.full((2,), 16, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    for total in (5.5, "5", None):
+        with pytest.raises(TypeError, match="total must be an int"):
+            flash_lab.gather_kv(kc, kc, lens, cu, total)
+    for total in (np.int64(5), 5):
+        with pytest.raises(ValueError, match="CUDA"):
+            flash_lab.gather_kv(kc, kc, lens, cu, total)
+
+
+@pytest.mark.gpu
+def test_gather_compiles_without_graph_breaks():
+    torch._dynamo.reset()
+    cache = Cache([64, 40], 2, 64, torch.bfloat16, True, page=16, poison=False)
+    cu = offsets([64, 40])
+
+    def read(kc, vc, lens, tables, ks, vs, total):
+        k, v = flash_lab.gather_kv(kc, vc, lens, cu, total, tables, ks, vs)
+        return k * 2, v
+
+    args = (cache.k, cache.v, cache.seq_lens, cache.block_tables, cache.scales["k_scale"],
+            cache.scales["v_scale"])
+    for total in (104, 110):
+        for got, want in zip(torch.compile(read, fullgraph=True)(*args, total), read(*args, total)):
+            assert torch.equal(got, want)
