@@ -12,12 +12,21 @@
 // scales. Weights below 2^-25 are 0 there (N of them make o differ by less than N 2^-18 steps of the row
 // with the largest weight); the sum of w_j / sv_j in fp32 keeps them.
 //
-// What bounds it. Every K/V byte is read once per 2 x 128 rows, so few rows per sequence are bound
+// What bounds it. An item of 2 x 128 rows reads its K/V bytes once, so few rows per sequence are bound
 // by HBM (2 H_kv D bytes per key at 8 bits, twice that at 16) and chunks of hundreds of rows by the
-// tensor cores and the exponentials. Measured on B200: 2048 rows after 16K bf16 keys (H 32, H_kv 8,
-// D 128) 468 us, 1.25 PFLOP/s; one row of 8 sequences of 24K bf16 keys (806 MB) 127 us, 6.3 TB/s;
-// prompts of 4 x 2500-4095 rows (fp16, 16 heads, D 64) 147 us, 0.57 PFLOP/s; the chunks of a mixed int8
-// batch about 0.45 PFLOP/s (its softmax takes 5000 clocks per tile where that of 16 bits takes 1800).
+// tensor cores and the exponentials. (Items of the same keys run at different times: 4 x 512 rows after
+// 16K keys, 8 items per KV head, read the K/V bytes 4 times from DRAM, the rest from L2.) Measured on
+// B200 as device time of a graph of two calls: 2048 rows after 16K bf16 keys (H 32, H_kv 8, D 128) 479 us,
+// 1.22 PFLOP/s (calls one after the other run at the power limit: 546-560 us, 1.04-1.07 PFLOP/s); one
+// row of 8 sequences of 24K bf16 keys (806 MB) 129 us, 6.3 TB/s; prompts of 4 x 2500-4095 rows
+// (fp16, 16 heads, D 64) 151 us, 0.56 PFLOP/s; 2 x 512 rows after 16K int8 keys (D 128) 467 us, 0.60
+// PFLOP/s (its softmax takes 5000 clocks per tile where that of 16 bits takes 1800).
+//
+// Roundings to fewer than 32 bits: the weights, to the type of the V operand of tcgen05.mma, which is the
+// cache's at 16 bits (bf16 2^-8, fp16 2^-11) and fp16 for codes; and the result, to q's type. Over bf16
+// caches that is 0.0021-0.0023 of the result's norm against 0.0016 with fp32 weights. Scores, reference
+// points, sums, O and the partials are fp32. log2 of a V scale is lg2.approx, off by at most 2^-22 of
+// itself.
 //
 // How it is split.
 //  * A tile of 128 score rows is (tokens x the query heads of one KV head): head h of token i is
@@ -341,14 +350,14 @@ __device__ __forceinline__ void weights_int8(uint32_t taddr_s, const float* scal
 // loop spilled, and the spills cost more than the softmax.
 //
 // A weight under 2^-126 is 0, and its term w / sv with it, however small sv is: a row of zeros in V has
-// sv = 2^-100. What a tile can lose that way is 128 terms under 2^-126 / sv, which is below 2^-32 of the
-// row's sum when the scales so far in the segment lie in [2^-40, 2^45] (a row that sees a key has a sum of
-// at least 1 / sv of one of them) or the sum is at least 2^13. Else the terms take exponentials of
-// their own.
+// sv = 2^-100. What a tile can lose that way is 128 terms under 2^-126 / sv. With scales in [2^-40, 2^45] so
+// far in the segment that is below 2^-34 of the row's sum, since a row that sees a key has a sum of at least
+// 1 / sv of one of them. With others it is below 2^-19, which over all tiles of the segment stays below 2^-20
+// of a sum of at least `need`, twice their number. Else the terms take exponentials of their own.
 template <int D>
 __device__ __forceinline__ void softmax_tile_int8(uint32_t taddr_s, uint32_t taddr_o,
-                                                  const float* scales, bool masked, int visible,
-                                                  float& m_ref, float& l_sum, uint64_t* bars,
+                                                  const float* scales, float need, bool masked,
+                                                  int visible, float& m_ref, float& l_sum, uint64_t* bars,
                                                   const PrevPv& prev, const WaitGuard& guard) {
   float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
@@ -383,7 +392,7 @@ __device__ __forceinline__ void softmax_tile_int8(uint32_t taddr_s, uint32_t tad
   const float nref = m_ref == -INFINITY ? 0.f : -m_ref;
   bool wide = false;
   if (reinterpret_cast<const int*>(scales)[Geometry<D, true>::kCareAt] != 0)   // of all rows alike
-    wide = __any_sync(0xffffffffu, mx != -INFINITY && !(l_sum >= 0x1p13f));
+    wide = __any_sync(0xffffffffu, mx != -INFINITY && !(l_sum >= need));
   float ps[4] = {0.f, 0.f, 0.f, 0.f};
   if (wide) {
     weights_int8<true>(taddr_s, scales, nref, ps, bars);
@@ -770,8 +779,8 @@ __global__ void __launch_bounds__(Geometry<D, kInt8>::kThreads, 1)
           }
           const float* scales = reinterpret_cast<const float*>(smem + G::kScaleOffset) +
                                 (at % G::kScaleSlots) * G::kScaleWords;
-          softmax_tile_int8<D>(taddr_s, taddr_o, scales, masked, limit - k0, m_ref, l_sum,
-                               sh->p_half[buf], prev, guard);
+          softmax_tile_int8<D>(taddr_s, taddr_o, scales, 2.f * count, masked, limit - k0, m_ref,
+                               l_sum, sh->p_half[buf], prev, guard);
         } else {
           softmax_tile<T, D>(taddr_s, taddr_o, a.scale_log2, masked, limit - k0, m_ref, l_sum,
                              sh->p_half[buf], prev, guard);

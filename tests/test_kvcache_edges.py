@@ -99,10 +99,13 @@ def test_extend_int8_rows_of_zeros_beside_large_ones(new, size, where, d):
     few-row kernel, 40 and 90 rows of 2 heads in items of one and of two tiles; a sequence has one to
     eight key tiles, and 60 sequences put several of them into a CTA.
 
-    The bounds of check_rows hold: log2 of a scale r, |r| <= 127, enters an exponent and leaves it
-    again, three roundings at magnitudes up to 256 (2^-17 ln 2 each), and the reference point and the
-    logarithm of the sum are two more at up to 128 (2^-18 each), together less than 2.4e-5: S is 6
-    and more, so (d + 8) 2^-24 S + 2^-19 alone is 2.7e-5."""
+    The bounds of check_rows hold. Where the terms of the sum take exponentials of their own, log2 of a
+    scale r, |r| <= 127, enters an exponent and leaves it again, three roundings at magnitudes up to
+    256 (2^-17 ln 2 each), and the reference point and the logarithm of the sum are two more at up to
+    128 (2^-18 each), together less than 2.4e-5. Where they do not, log2 2^-100 is off by at most
+    100 * 2^-22 and its exponent by two roundings (2^-18 and 2^-17), all times ln 2, and the sum by 2^-20
+    of it: less than 2.6e-5.
+    S is 6 and more, so (d + 8) 2^-24 S + 2^-19 alone is 2.7e-5."""
     rng = np.random.RandomState(11)
     lens = [int(x) for x in rng.randint(new + 30, 300, 60)] + [1000]
     steps = np.concatenate([size * 2.0 ** -rng.randint(0, 3, n).astype(np.float64) if size > 1 else
