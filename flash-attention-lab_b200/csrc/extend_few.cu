@@ -3,7 +3,8 @@
 // and partials as extend.cu; HBM bound (2 H_kv (D + 4) bytes per key), so the codes go from shared
 // memory straight into the registers of 16 x 8 x 16 warp MMAs instead of through 16-bit tiles. One
 // row of 8 sequences of 24K keys, 32 query and 8 KV heads, D 128 (415 MB): 80 us with the merge,
-// 5.2 TB/s; the first tcgen05 form of extend.cu took 297 us.
+// 5.2 TB/s; the first tcgen05 form of extend.cu took 297 us. Roundings to fewer than 32 bits: bf16 queries
+// to fp16 (below), the weights to fp16, the result to q's type.
 //
 //  * One CTA per SM: two warps stream [128 keys x D] tiles of K and of V codes by TMA, one turns the
 //    keys' scales into what the scores need (below) beside them in the ring stage, and eight consumer

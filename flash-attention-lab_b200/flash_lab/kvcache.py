@@ -290,7 +290,8 @@ def extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seq_le
     query heads per KV head. A non-finite value in V makes the whole tile of up to 128 keys around
     it non-finite for every row that reads the tile, also for rows that the causal mask keeps from
     that key (int8 caches: only for the rows that see it); keys at or past seq_lens[b] are never
-    read into a result.
+    read into a result. A call gives the same bits each time; over an int8 cache the same rows given with
+    cu_seqlens and without it may be worked by different kernels and differ in their last bits.
     """
     out, lse = _extend_checked(0, q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, causal,
                                softmax_scale, k_scale, v_scale)

@@ -281,8 +281,10 @@ int flb_peer_exchange_reset(const flb_peer_exchange* exchange, flb_stream_t stre
  * k_batch_stride the block stride, max_seqlen = max_blocks * page_size).
  * dtype FLB_INT8: row x of D values (one token, one KV head) is stored as the codes
  * q = round(x * min(127 / max|x|, 2^100)) (to nearest even) and the fp32 scale
- * s = max(max|x| / 127, 2^-100), and stands for q * s. A row with a non-finite value is stored as
- * zeros with a NaN scale and reads back as NaN. k_scale / v_scale hold one scale per token and KV
+ * s = min(max(max|x| / 127, 2^-100), 2^121 * 1.0079), the bounds of which keep 127 s finite, and stands
+ * for q * s; 1 / max|x|, 1 / 127 and the products are rounded to fp32. A row with a non-finite value is
+ * stored as zeros with a NaN scale and reads back as NaN. flb_extend_fwd reads V scales below 2^-100 as
+ * 2^-100 and V scales above 2^127 as NaN. k_scale / v_scale hold one scale per token and KV
  * head, [B, S_max, H_kv] (or [num_blocks, page_size, H_kv]) with any strides; NULL otherwise.
  * All strides are in elements.
  */
