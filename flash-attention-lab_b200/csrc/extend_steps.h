@@ -20,6 +20,8 @@
 //   x_ready/done  Once per joined segment, waited for each time by the other chain.
 //   q, k, v       Rings whose two sides wait for every phase. A chain also waits for the v_empty of its
 //                 previous step's tile, see PrevPv.
+//   scale_full[s] The converter of K writes a tile's scales before the tile, so s_full of the step says that
+//                 they are there; their place is taken again only once the readers are done (kScaleSlots).
 //   code_full[s]  The tiles of one place belong to K and V by turns, and copies land in any order: a
 //                 converter that waits for its tile knows nothing of the one before, which is the
 //                 other's. So it waits for that tile's release first. Its own comes next, so the

@@ -5,6 +5,7 @@
 // violation, and so is a state from which no role can go on.
 //
 //   extend_protocol softmax RULE    RULE joined: as the kernel; dual: only one-tile segments joined
+//   extend_protocol scales RULE     RULE kept: as the kernel; fewer: the scales of one key tile less are held
 //   extend_protocol codes RULE      RULE release: as the kernel; full: converters wait for code_full alone
 //
 // Prints the number of sequences and of states, or the first violation (exit 1).
@@ -21,9 +22,10 @@ using flb::Steps;
 
 namespace {
 
+enum class Kind { kWait, kArrive, kNeeds };
 struct Op {
-  bool wait;
-  int bar, phase;   // wait: for this phase; else one more phase of the barrier completes
+  Kind kind;
+  int bar, phase;   // wait for this phase; one more phase completes; that many have completed, or it is a fault
 };
 using Program = std::vector<Op>;
 struct Model {
@@ -37,9 +39,14 @@ struct Model {
     return static_cast<int>(bars.size()) - 1;
   }
   void wait(int role, const std::string& name, int phase) {
-    roles[role].push_back({true, bar(name), phase});
+    roles[role].push_back({Kind::kWait, bar(name), phase});
   }
-  void arrive(int role, const std::string& name) { roles[role].push_back({false, bar(name), 0}); }
+  void arrive(int role, const std::string& name) {
+    roles[role].push_back({Kind::kArrive, bar(name), 0});
+  }
+  void needs(int role, const std::string& name, int phases) {
+    roles[role].push_back({Kind::kNeeds, bar(name), phases});
+  }
 };
 
 struct Result {
@@ -56,7 +63,7 @@ Result explore(const Model& m) {
     done[r].assign(m.roles[r].size() + 1, std::vector<int>(bars, 0));
     for (size_t i = 0; i < m.roles[r].size(); ++i) {
       done[r][i + 1] = done[r][i];
-      if (!m.roles[r][i].wait) ++done[r][i + 1][m.roles[r][i].bar];
+      if (m.roles[r][i].kind == Kind::kArrive) ++done[r][i + 1][m.roles[r][i].bar];
     }
   }
   Result result;
@@ -82,10 +89,15 @@ Result explore(const Model& m) {
       if (at == m.roles[r].size()) continue;
       ended = false;
       const Op& op = m.roles[r][at];
-      if (op.wait) {
+      if (op.kind != Kind::kArrive) {
         int completed = 0;
         for (size_t q = 0; q < roles; ++q) completed += done[q][place(s, q)][op.bar];
-        if (completed < op.phase || completed > op.phase + 1) {
+        if (op.kind == Kind::kNeeds) {
+          if (completed < op.phase) {
+            result.error = "role " + std::to_string(r) + " goes on before " + m.bars[op.bar];
+            return result;
+          }
+        } else if (completed < op.phase || completed > op.phase + 1) {
           char text[160];
           std::snprintf(text, sizeof(text), "role %zu waits for phase %d of %s, %d completed", r,
                         op.phase, m.bars[op.bar].c_str(), completed);
@@ -93,7 +105,7 @@ Result explore(const Model& m) {
           result.error = text;
           return result;
         }
-        if (completed == op.phase) continue;
+        if (op.kind == Kind::kWait && completed == op.phase) continue;
       }
       moved = true;
       const uint64_t next = s + (uint64_t{1} << (bits * r));
@@ -111,11 +123,14 @@ std::string numbered(const char* name, int i) { return name + std::to_string(i);
 
 // Roles: 0 the MMA lane, 1 the tensor cores (they work in order, a commit completes what came
 // before it), 2 and 3 the softmax warpgroups. K, V and Q are always there. rescale: every step moves
-// its reference point, which is when a chain waits for P V of its previous step.
+// its reference point, which is when a chain waits for P V of its previous step. With scale_slots > 0 also
+// 4, the converter of K, which writes the scales of a tile into one of so many places before the tile.
 Model softmax_model(const std::vector<Steps>& segments, int s_bufs, int v_slots, bool rescale,
-                    bool join_count0) {
+                    bool join_count0, int k_slots = 0, int scale_slots = 0) {
   Model m;
-  m.roles.resize(4);
+  m.roles.resize(scale_slots > 0 ? 5 : 4);
+  std::vector<int> readers[2];   // steps that each chain has done once it has read the tile's scales
+  int chain_steps[2] = {0, 0};
   int n_base = 0, kv_base = 0, p_waits[3] = {0, 0, 0}, o_waits[2] = {0, 0}, joins = 0, issued = 0;
   for (const Steps& s : segments) {
     const int steps = s.count0 + s.count1;
@@ -128,11 +143,30 @@ Model softmax_model(const std::vector<Steps>& segments, int s_bufs, int v_slots,
       ++issued;
       m.arrive(1, bar);
     };
-    auto qk = [&](int i) { tensor(numbered("s_full", (n_base + i) % s_bufs)); };
+    auto entry_of = [&](int i) {
+      return kv_base + (i < s.paired() ? (s.dual ? i : i >> 1) : i - s.count0);
+    };
+    auto qk = [&](int i) {
+      const int entry = entry_of(i);
+      if (scale_slots > 0) m.wait(0, numbered("k_full", entry % k_slots), entry / k_slots);
+      tensor(numbered("s_full", (n_base + i) % s_bufs));
+      if (scale_slots > 0 && (s.dual || s.chain(i) == 1)) tensor(numbered("k_empty", entry % k_slots));
+    };
+    for (int c = 0; c < 2; ++c) {
+      readers[c].resize(kv_base + tiles, chain_steps[c]);
+      for (int j = 0; j < s.count(c); ++j) readers[c][kv_base + s.place(c, j)] = ++chain_steps[c];
+    }
+    for (int at = kv_base; scale_slots > 0 && at < kv_base + tiles; ++at) {
+      if (at >= k_slots) m.wait(4, numbered("k_empty", at % k_slots), at / k_slots - 1);
+      for (int c = 0; c < 2 && at >= scale_slots; ++c)   // who read the place's last scales has done so
+        m.needs(4, numbered("step", c), readers[c][at - scale_slots]);
+      m.arrive(4, numbered("scale_full", at % scale_slots));
+      m.arrive(4, numbered("k_full", at % k_slots));
+    }
     for (int i = 0; i < s_bufs && i < steps; ++i) qk(i);
     for (int i = 0; i < steps; ++i) {
       const int c = s.chain(i), buf = (n_base + i) % s_bufs;
-      const int entry = kv_base + (i < s.paired() ? (s.dual ? i : i >> 1) : i - s.count0);
+      const int entry = entry_of(i);
       m.wait(0, numbered("p", buf), p_waits[buf]++);
       if (s.dual || c == 1) tensor(numbered("v_empty", entry % v_slots));
       if (i == s.other_last() || i == steps - 1) tensor(numbered("o_full", c));
@@ -146,6 +180,11 @@ Model softmax_model(const std::vector<Steps>& segments, int s_bufs, int v_slots,
         if (rescale && j > 0 && s.order(c, j) - s.order(c, j - 1) < s_bufs) {
           const int v = kv_base + s.place(c, j - 1);
           m.wait(role, numbered("v_empty", v % v_slots), v / v_slots);
+        }
+        if (scale_slots > 0) {
+          const int at = kv_base + s.place(c, j);
+          m.wait(role, numbered("scale_full", at % scale_slots), at / scale_slots);
+          m.arrive(role, numbered("step", c));
         }
         m.arrive(role, numbered("p", n % s_bufs));
       }
@@ -215,6 +254,24 @@ bool softmax(bool join_count0) {
   return true;
 }
 
+bool scales(int held_less) {
+  std::vector<Steps> kinds;
+  for (int n : {1, 2, 5}) kinds.push_back({true, (n + 1) / 2, n / 2});
+  for (int n : {0, 1, 3}) kinds.push_back({false, n, n + 1});
+  kinds.push_back({false, 4, 4});
+  const int shapes[2][3] = {{2, 1, 2}, {3, 2, 4}};   // S buffers, V and K places at head_dim 128 and 64
+  for (const auto& shape : shapes) {
+    for (const Steps& a : kinds) {
+      for (const Steps& b : kinds) {
+        const Model m = softmax_model({a, b, a}, shape[0], shape[1], false, true, shape[2],
+                                      shape[2] + shape[0] - held_less);
+        if (!check(m, std::to_string(shape[0]) + " S buffers")) return false;
+      }
+    }
+  }
+  return true;
+}
+
 // Roles: 0 the producer, 1 and 2 the converters of K and V, then one for each place of the ring, whose
 // copies land at any time after their issue, in any order among places.
 Model codes_model(const std::vector<int>& tiles, int slots, bool wait_release) {
@@ -265,10 +322,12 @@ int main(int argc, char** argv) {
   bool ok;
   if (part == "softmax" && (rule == "joined" || rule == "dual")) {
     ok = softmax(rule == "joined");
+  } else if (part == "scales" && (rule == "kept" || rule == "fewer")) {
+    ok = scales(rule == "fewer");
   } else if (part == "codes" && (rule == "release" || rule == "full")) {
     ok = codes(rule == "release");
   } else {
-    std::printf("usage: extend_protocol softmax joined|dual, or codes release|full\n");
+    std::printf("usage: extend_protocol softmax joined|dual, scales kept|fewer, or codes release|full\n");
     return 2;
   }
   if (ok) std::printf("%ld sequences, %ld states\n", sequences, states);

@@ -35,6 +35,13 @@ def test_softmax_warpgroups_never_wait_for_a_phase_two_ahead(model):
     assert code == 1 and "two-tile(0, 1) two-tile(0, 1)" in text and "s_full" in text
 
 
+def test_scales_are_not_overwritten_while_they_are_read(model):
+    code, text = model("scales", "kept")
+    assert code == 0, text
+    code, text = model("scales", "fewer")
+    assert code == 1 and "goes on before step" in text
+
+
 def test_converters_never_wait_for_a_phase_two_ahead(model):
     code, text = model("codes", "release")
     assert code == 0, text
